@@ -187,7 +187,13 @@ mod ffi {
         pub fn tm_cuda_attention_decode_batch_dev(ctx: *mut TmCudaCtx, q: *mut TmCudaBuffer, k: *mut TmCudaBuffer, v: *mut TmCudaBuffer, q_norm: *mut TmCudaBuffer, k_norm: *mut TmCudaBuffer, inv_freq: *mut TmCudaBuffer, k_cache: *mut TmCudaBuffer, v_cache: *mut TmCudaBuffer, out: *mut TmCudaBuffer, scratch: *mut TmCudaBuffer, pos_buf: *mut TmCudaBuffer, status: *mut TmCudaBuffer, n_seq: u32, q_stride: u32, kv_stride: u32, heads: u32, kv_heads: u32, head_dim: u32, n_rot: u32, cap: u32, window: u32, eps: f32, scale: f32, exact: c_int, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_rows_indirect_seq_f32_dev(ctx: *mut TmCudaCtx, w: *mut TmCudaBuffer, rows: u32, cols: u32, ids: *mut TmCudaBuffer, ids_stride: u32, pos_buf: *mut TmCudaBuffer, n_seq: u32, bias: i32, scale: f32, out: *mut TmCudaBuffer, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_argmax_rows_f32_dev(ctx: *mut TmCudaCtx, x: *mut TmCudaBuffer, n_rows: u32, n: u32, partial: *mut TmCudaBuffer, out: *mut TmCudaBuffer, out_stride: u32, base: u32, pos_buf: *mut TmCudaBuffer, out_cap: u32, mirror: *mut TmCudaBuffer, err: *mut c_char, err_cap: usize) -> c_int;
+        pub fn tm_cuda_logits_adjust_rows_f32_dev(ctx: *mut TmCudaCtx, x: *mut TmCudaBuffer, y: *mut TmCudaBuffer, n_rows: u32, n: u32, log: *mut TmCudaBuffer, log_stride: u32, base: u32, pos_buf: *mut TmCudaBuffer, log_cap: u32, prompt_len: *mut TmCudaBuffer, penalties: *mut TmCudaBuffer, bias_ids: *mut TmCudaBuffer, bias_values: *mut TmCudaBuffer, bias_count: *mut TmCudaBuffer, bias_cap: u32, mask: *mut TmCudaBuffer, partial: *mut TmCudaBuffer, mirror: *mut TmCudaBuffer, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_u32_add_sat(ctx: *mut TmCudaCtx, buf: *mut TmCudaBuffer, first: u32, count: u32, delta: u32, limit: u32, err: *mut c_char, err_cap: usize) -> c_int;
+        pub fn tm_cuda_kv_pages_supported(head_dim: u32, page_rows: u32) -> c_int;
+        pub fn tm_cuda_attention_paged_scratch_bytes(n_seq: u32, heads: u32, kv_heads: u32, head_dim: u32, page_rows: u32, max_pages: u32, weights: c_int) -> usize;
+        pub fn tm_cuda_attention_decode_paged_dev(ctx: *mut TmCudaCtx, q: *mut TmCudaBuffer, k: *mut TmCudaBuffer, v: *mut TmCudaBuffer, q_norm: *mut TmCudaBuffer, k_norm: *mut TmCudaBuffer, inv_freq: *mut TmCudaBuffer, k_pages: *mut TmCudaBuffer, v_pages: *mut TmCudaBuffer, table: *mut TmCudaBuffer, out: *mut TmCudaBuffer, scratch: *mut TmCudaBuffer, pos_buf: *mut TmCudaBuffer, len_buf: *mut TmCudaBuffer, status: *mut TmCudaBuffer, weights_in: *mut TmCudaBuffer, weights_out: *mut TmCudaBuffer, n_seq: u32, q_stride: u32, kv_stride: u32, heads: u32, kv_heads: u32, head_dim: u32, n_rot: u32, pages: u32, page_rows: u32, max_pages: u32, window: u32, eps: f32, scale: f32, err: *mut c_char, err_cap: usize) -> c_int;
+        pub fn tm_cuda_kv_pages_copy_f16(ctx: *mut TmCudaCtx, k_cache: *mut TmCudaBuffer, v_cache: *mut TmCudaBuffer, k_pages: *mut TmCudaBuffer, v_pages: *mut TmCudaBuffer, table: *mut TmCudaBuffer, status: *mut TmCudaBuffer, pages: u32, page_rows: u32, max_pages: u32, kv_heads: u32, head_dim: u32, cap: u32, to_pages: c_int, n_runs: u32, runs: *const u32, err: *mut c_char, err_cap: usize) -> c_int;
+        pub fn tm_cuda_kv_pages_evict(ctx: *mut TmCudaCtx, k_pages: *mut TmCudaBuffer, v_pages: *mut TmCudaBuffer, table: *mut TmCudaBuffer, to_table: *mut TmCudaBuffer, len_buf: *mut TmCudaBuffer, len_out: *mut TmCudaBuffer, weights: *mut TmCudaBuffer, weights_out: *mut TmCudaBuffer, kept: *mut TmCudaBuffer, status: *mut TmCudaBuffer, n_seq: u32, kv_heads: u32, head_dim: u32, pages: u32, page_rows: u32, max_pages: u32, keep: u32, first: u32, recent: u32, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_u32_add(ctx: *mut TmCudaCtx, buf: *mut TmCudaBuffer, index: u32, delta: u32, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_argmax_f32_dev(ctx: *mut TmCudaCtx, x: *mut TmCudaBuffer, n: u32, partial: *mut TmCudaBuffer, out: *mut TmCudaBuffer, base: u32, pos_buf: *mut TmCudaBuffer, pos_index: u32, out_cap: u32, mirror: *mut TmCudaBuffer, err: *mut c_char, err_cap: usize) -> c_int;
         pub fn tm_cuda_row_indirect_f32_dev(ctx: *mut TmCudaCtx, w: *mut TmCudaBuffer, rows: u32, cols: u32, ids: *mut TmCudaBuffer, base: u32, pos_buf: *mut TmCudaBuffer, pos_index: u32, bias: i32, scale: f32, out: *mut TmCudaBuffer, err: *mut c_char, err_cap: usize) -> c_int;

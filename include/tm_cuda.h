@@ -635,10 +635,91 @@ int tm_cuda_argmax_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, uint32_t n_
                                 tm_cuda_buffer *partial, tm_cuda_buffer *out, uint32_t out_stride, uint32_t base,
                                 tm_cuda_buffer *pos_buf, uint32_t out_cap, tm_cuda_buffer *mirror, char *err,
                                 size_t err_cap);
+/* No counterpart: the logits of a decode step before a token is chosen; y (x itself, or other storage) for n_rows rows
+ * of n logits, each step rounded to f32:
+ *   penalties (may be NULL)  f32 [n_rows][3]: repetition, presence, frequency.  A token that the row's log holds below the
+ *                            slot base + pos_buf[r] (at most log_cap entries) is divided by `repetition` where its logit is
+ *                            positive, else multiplied by it; one that the log holds c > 0 times from entry prompt_len[r] on
+ *                            (NULL: 0) then loses frequency * c and presence.  Ids >= n in a log are no token.
+ *   bias_ids / _values / _count (all or none)  u32 and f32 [n_rows][bias_cap], of which min(bias_count[r], bias_cap) count:
+ *                            value added to the id's logit; of entries with one id the last, an id >= n none.
+ *   mask (may be NULL)       [n_rows][ceil(n / 32)] words; bit t % 32 of word t / 32 clear: -infinity.
+ * With `partial` (n_rows * TM_CUDA_LOGITS_PARTIAL_BYTES) each row's largest logit that is neither masked nor NaN (ties to
+ * the lowest index, 0xFFFFFFFF when there is none) goes to log[r * log_stride + base + pos_buf[r]], and to `mirror` when
+ * given, if that slot is below log_cap <= log_stride.  n <= TM_CUDA_LOGITS_MAX.  Refused where an operand that is written
+ * shares storage with another, but for y with x. */
+#define TM_CUDA_LOGITS_MAX (1u << 21)
+#define TM_CUDA_LOGITS_PARTIAL_BYTES 2048
+int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_cuda_buffer *y, uint32_t n_rows, uint32_t n,
+                                       tm_cuda_buffer *log, uint32_t log_stride, uint32_t base, tm_cuda_buffer *pos_buf,
+                                       uint32_t log_cap, tm_cuda_buffer *prompt_len, tm_cuda_buffer *penalties,
+                                       tm_cuda_buffer *bias_ids, tm_cuda_buffer *bias_values, tm_cuda_buffer *bias_count,
+                                       uint32_t bias_cap, tm_cuda_buffer *mask, tm_cuda_buffer *partial,
+                                       tm_cuda_buffer *mirror, char *err, size_t err_cap);
 /* buf[first + i] = min(buf[first + i] + delta, limit), i < count: advances every sequence's position;
  * a sequence that has filled its cache stays on its last row instead of running past it. */
 int tm_cuda_u32_add_sat(tm_cuda_ctx *ctx, tm_cuda_buffer *buf, uint32_t first, uint32_t count, uint32_t delta,
                         uint32_t limit, char *err, size_t err_cap);
+/* ---- a pool of cache pages shared by many sequences (no counterpart) ----
+ * Pools are f16 [pages][kv_heads][page_rows][head_dim]; row j of sequence s lies in page table[s * max_pages + j / page_rows],
+ * row j % page_rows; a sequence has up to max_pages * page_rows rows.  head_dim 32, 64, 128 or 256; page_rows 16, 32, 64,
+ * 128 or 256 (`supported`); pages * kv_heads * page_rows < 2^32, kv_heads <= 4096, max_pages * page_rows <= 2^25.  Sequences may share
+ * pages that nothing writes.  A page id >= pages (an entry of a page that is not there) that a call would use sets bit 2
+ * of status[0]: its rows are read as zeros and nothing is stored to it.  Entries of pages that a call does not use (behind
+ * the last row, wholly before a window) are not looked at.  Tables, lengths and positions are device memory, read when the
+ * operator runs, so that a recorded graph serves every step.  Operands that a call writes may share no storage with its
+ * others, except where it says so: such a call is refused. */
+#define TM_CUDA_STATUS_BAD_PAGE 4u
+#define TM_CUDA_SEQ_NONE 0xffffffffu
+#define TM_CUDA_PAGED_MAX_SEQUENCES 1024u
+int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows);
+/* Decode attention of one new token for each of n_seq (<= TM_CUDA_PAGED_MAX_SEQUENCES) sequences over its pages: the paged
+ * form of tm_cuda_attention_decode_batch_dev, with 32-bit accuracy (queries and softmax weights are held as sums of two
+ * f16).  The new key, normed and rotated at position pos_buf[s], and the new value are stored at row len_buf[s], and the
+ * token attends rows start .. len_buf[s], start = len + 1 > window ? len + 1 - window : 0 (window 0: all).  The two buffers
+ * may be one; they differ once rows have been evicted, and a window then counts rows.  Rows of q start q_stride elements
+ * apart, of k and v kv_stride (0 = dense); out is [n_seq][heads * head_dim]; heads / kv_heads <= 32.
+ * weights_out (may be NULL): [n_seq][kv_heads][max_pages * page_rows] f32, the attention that each row has drawn:
+ * weights_in (NULL: zeros; may be weights_out) plus the sum of the softmax weights that the KV head's query heads give it
+ * now.  The new row starts from 0; entries behind it are left as they are.
+ * A length of TM_CUDA_SEQ_NONE: the sequence takes no part, nothing of it is written.  A length >= max_pages * page_rows:
+ * the same, and bit 0 of status[0] is set.  An infinity or NaN in a row in sight makes the heads that read it NaN; rows out
+ * of sight have no effect.  scratch holds tm_cuda_attention_paged_scratch_bytes and needs no clearing; calls that share it
+ * must be ordered on the stream. */
+size_t tm_cuda_attention_paged_scratch_bytes(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                             uint32_t page_rows, uint32_t max_pages, int weights);
+int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_cuda_buffer *k, tm_cuda_buffer *v,
+                                       tm_cuda_buffer *q_norm, tm_cuda_buffer *k_norm, tm_cuda_buffer *inv_freq,
+                                       tm_cuda_buffer *k_pages, tm_cuda_buffer *v_pages, tm_cuda_buffer *table,
+                                       tm_cuda_buffer *out, tm_cuda_buffer *scratch, tm_cuda_buffer *pos_buf,
+                                       tm_cuda_buffer *len_buf, tm_cuda_buffer *status, tm_cuda_buffer *weights_in,
+                                       tm_cuda_buffer *weights_out, uint32_t n_seq, uint32_t q_stride, uint32_t kv_stride,
+                                       uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n_rot,
+                                       uint32_t pages, uint32_t page_rows, uint32_t max_pages, uint32_t window, float eps,
+                                       float scale, char *err, size_t err_cap);
+/* Copies runs of rows between dense planes [sequences][kv_heads][cap][head_dim] (what prefill writes and reads) and pages:
+ * runs holds (dense sequence, table row, first row, rows) per run, at most TM_CUDA_PREFILL_SEGMENTS; row j of the dense
+ * sequence is row j of the paged one.  to_pages: into the pages, else out of them.  Two runs that store the same rows are
+ * refused. */
+int tm_cuda_kv_pages_copy_f16(tm_cuda_ctx *ctx, tm_cuda_buffer *k_cache, tm_cuda_buffer *v_cache, tm_cuda_buffer *k_pages,
+                              tm_cuda_buffer *v_pages, tm_cuda_buffer *table, tm_cuda_buffer *status, uint32_t pages,
+                              uint32_t page_rows, uint32_t max_pages, uint32_t kv_heads, uint32_t head_dim, uint32_t cap,
+                              int to_pages, uint32_t n_runs, const uint32_t *runs, char *err, size_t err_cap);
+/* Evicts rows by the attention they have drawn: of each sequence with len_buf[s] > keep, every KV head keeps its first
+ * `first` rows, its last `recent` rows and, of those between, the ones with the largest weights (ties to the lower row,
+ * NaN last), `keep` in all, in their order.  Kept row i of a head moves to row i of to_table's pages, kept[s][h][i] (u32,
+ * [n_seq][kv_heads][keep]) receives its number and weights_out[s][h][i] its weight (layout of the attention operator's;
+ * may be `weights` itself, entries behind are left as they are); len_out[s] (may be len_buf itself) receives keep.  A
+ * sequence with at most keep rows keeps all of them: kept[s][h][i] = i below its length and 0xFFFFFFFF behind.
+ * to_table is `table` itself (the rows move down in place; no page may then be shared) or names pages that no
+ * sequence reads from.  A length of TM_CUDA_SEQ_NONE, or one > max_pages * page_rows (which sets bit 0 of
+ * status[0]): nothing of the sequence is written, len_out receives the length as it is. */
+int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_buffer *v_pages, tm_cuda_buffer *table,
+                           tm_cuda_buffer *to_table, tm_cuda_buffer *len_buf, tm_cuda_buffer *len_out,
+                           tm_cuda_buffer *weights, tm_cuda_buffer *weights_out, tm_cuda_buffer *kept,
+                           tm_cuda_buffer *status, uint32_t n_seq, uint32_t kv_heads, uint32_t head_dim, uint32_t pages,
+                           uint32_t page_rows, uint32_t max_pages, uint32_t keep, uint32_t first, uint32_t recent, char *err,
+                           size_t err_cap);
 /* No counterpart: buf[index] += delta (u32), to advance a device position
  * inside a recorded graph. */
 int tm_cuda_u32_add(tm_cuda_ctx *ctx, tm_cuda_buffer *buf, uint32_t index, uint32_t delta,

@@ -195,6 +195,25 @@ inline void tm_settle(tm_cuda_ctx *ctx) { ctx->settled = ctx->op - 1; }
         tm_read_ahead(ctx, (buf));                                           \
     } while (0)
 
+// Operands of one call, to refuse storage that one of them writes and another reads or writes.  Operands `same_a` and `same_b`
+// may be the same storage, as a whole.
+struct tm_span {
+    const tm_cuda_buffer *b;  // none: not given
+    size_t bytes;
+    bool written;
+    const char *what;
+};
+inline int tm_check_disjoint(const tm_span *s, size_t n, size_t same_a, size_t same_b, char *err, size_t err_cap) {
+    for (size_t i = 0; i < n; ++i)
+        for (size_t j = i + 1; j < n; ++j) {
+            if (!s[i].b || !s[j].b || !(s[i].written || s[j].written)) continue;
+            if (s[i].b->dev >= s[j].b->dev + s[j].bytes || s[j].b->dev >= s[i].b->dev + s[i].bytes) continue;
+            if (i == same_a && j == same_b && s[i].b->dev == s[j].b->dev) continue;
+            return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "operands share storage: %s, %s", s[i].what, s[j].what);
+        }
+    return TM_CUDA_OK;
+}
+
 // Every operator entry point opens with this: context present, device current,
 // dispatch serialised (crates/metal/src/lib.rs:695-707 holds a mutex the same way).
 #define TM_ENTER()                                                                          \

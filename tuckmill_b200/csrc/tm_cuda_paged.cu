@@ -1,0 +1,1034 @@
+// A pool of cache pages shared by many sequences: decode attention over it, copies between it and the dense planes of
+// prefill, and the eviction of rows that drew little attention.
+//
+// Pools are [pages][kv_heads][page_rows][head_dim] f16.  Row j of sequence s lies in page table[s][j / page_rows]; a
+// row is contiguous, and the rows of one head in one page are.  Every page id is compared with the number of pages
+// before it becomes an address: an id that is none reads as zeros, is not written, and sets TM_CUDA_STATUS_BAD_PAGE.
+#include "tm_cuda_internal.cuh"
+#include "tm_cuda_device.cuh"
+
+namespace {
+
+using tmdev::mma_f16;
+using tmdev::smem_addr;
+
+constexpr uint32_t kSeqNone = TM_CUDA_SEQ_NONE;
+
+bool pages_ok(uint32_t head_dim, uint32_t page_rows) {
+    return (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+           (page_rows == 16 || page_rows == 32 || page_rows == 64 || page_rows == 128 || page_rows == 256);
+}
+uint32_t log2_of(uint32_t v) {
+    uint32_t l = 0;
+    while ((1u << l) < v) ++l;
+    return l;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {  // zeros where not live
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+// Byte offset of 16-byte chunk `chunk` of row `row` in rows of PITCH bytes: the eight rows that an ldmatrix reads at one
+// chunk fall into distinct banks.
+template <int PITCH>
+__device__ __forceinline__ uint32_t sw(uint32_t row, uint32_t chunk) {
+    if (PITCH >= 128) return row * PITCH + ((chunk ^ (row & 7u)) << 4);
+    return row * PITCH + ((chunk ^ ((row >> 1) & 3u)) << 4);  // 64-byte rows: two rows per 128 bytes
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+
+// ---- decode attention ------------------------------------------------------------------------------
+//
+// One new token of every sequence: z_hj = scale q_h . k_j over the rows j in sight, P = softmax(z), out_h = sum_j P_hj v_j,
+// and, where a caller counts attention, weights[kv][j] += sum over the group's heads of P_hj.
+//
+// What bounds it: the cached rows' bytes, 4 head_dim per row and KV head.  So every row is read once for all (up to
+// eight) query heads of its group, and the machine's bandwidth is shared out evenly however ragged the lengths are:
+// the tiles of 64 rows of all (sequence, KV head) pairs form one line, and CTA i of G takes the i-th of G equal runs of
+// it.  A pair that falls into one run is finished there; pieces of the others meet in a second, small launch.
+//
+// A warp takes 16 rows of each tile through its own ring of cp.async stages and keeps its own running (max, sum, output),
+// so the warps of a CTA do not meet before the end of a run.  Both products are mma.m16n8k16 with the cached rows as the
+// 16-row operand and the heads as the 8 columns: S^T = K Q^T, then O^T = V^T P^T, with P transposed in registers.
+//
+// Accuracy: cached rows are f16, so their products with f16 operands are exact in f32.  Q and P are split into a sum of two
+// f16 each (22 bits; Q against a power of two at its largest element, P in units of 2^-14, so that neither runs out of
+// exponents), and every product of a 16-row step starts from zero and is added to the f32 sums by a fused multiply-add:
+// results are those of 32-bit arithmetic.  The second multiply hides behind the loads.
+constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
+constexpr uint32_t kBlock = 16, kTile = kBlock * kAttnWarps;
+constexpr uint32_t kMostCtas = 640;
+constexpr float kUnit = 14.0f;  // P and its sums are held times 2^14
+
+template <int HD>
+struct attn_cfg {
+    static constexpr int PITCH = HD * 2;
+    static constexpr uint32_t kPlane = kBlock * PITCH, kStage = 2 * kPlane;  // a warp's 16 keys, then its 16 values
+    static constexpr int kStages = HD > 64 ? 3 : 4;
+    static constexpr int kCtas = HD == 256 ? 1 : HD == 128 ? 2 : 3;  // an SM
+    static constexpr int QP = HD + 8;                                // halves a row of Q: distinct banks for 8 rows
+    static constexpr uint32_t kRing = kAttnWarps * kStages * kStage;
+    static constexpr uint32_t kBytes = kRing + 2 * 8 * QP * 2 + 2 * HD * 2 + 9 * HD * 4 + (8 + 2 * kAttnWarps * 8) * 4;
+};
+
+struct paged_args {
+    const float *q, *k, *v, *q_norm, *k_norm, *inv_freq;
+    __half *kp, *vp;
+    const uint32_t *table, *pos, *len;
+    float *out, *part, *scores, *ml;  // scores, ml: only where weights are counted
+    const float *w_in;
+    float *w_out;
+    uint32_t *status;
+    uint32_t n_seq, q_stride, kv_stride, heads, kv_heads, group, blocks;  // blocks of up to 8 heads in a group
+    uint32_t n_rot, pages, page_log, max_pages, cap, window, ctas;
+    float eps, scale_log2e;
+};
+
+__device__ __forceinline__ uint32_t first_row(uint32_t len, uint32_t window) {
+    return window != 0u && len >= window ? len + 1u - window : 0u;
+}
+// Tiles of one (sequence, KV head) pair; none for a sequence that takes no part or is full.
+__device__ __forceinline__ uint32_t pair_tiles(uint32_t len, const paged_args &a) {
+    return len >= a.cap ? 0u : len / kTile - first_row(len, a.window) / kTile + 1u;
+}
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Tiles of all sequences' pairs before sequence `upto` (whole warps call it).
+__device__ __forceinline__ uint64_t tiles_before(uint32_t upto, const paged_args &a) {
+    uint64_t n = 0;
+    for (uint32_t s = threadIdx.x & 31u; s < upto; s += 32u) n += pair_tiles(a.len[s], a);
+    return warp_sum(n) * (a.kv_heads * a.blocks);
+}
+// The CTAs that share T tiles: each has one at least, so the pieces of a pair lie in consecutive CTAs.
+__device__ __forceinline__ uint32_t sharers(uint64_t T, const paged_args &a) { return (uint32_t)min(T, (uint64_t)a.ctas); }
+// Which CTA owns tile t of T: the i with i T / G <= t < (i + 1) T / G, whole numbers throughout.
+__device__ __forceinline__ uint32_t cta_of(uint64_t t, uint64_t T, uint32_t G) { return (uint32_t)(((t + 1) * G - 1) / T); }
+
+template <int HD>
+__global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_paged_kernel(const paged_args a) {
+    using C = attn_cfg<HD>;
+    constexpr int PITCH = C::PITCH, STAGES = C::kStages, QP = C::QP, EPL = HD / 32;
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char *ring = smem;
+    __half *q_hi = (__half *)(smem + C::kRing), *q_lo = q_hi + 8 * QP;
+    __half *k_new = q_lo + 8 * QP, *v_new = k_new + HD;
+    float *vec = (float *)(v_new + HD);  // a head vector per warp and iteration, for the rotation's pairs
+    float *factor = vec + 9 * HD, *wm = factor + 8, *wl = wm + kAttnWarps * 8;
+    const uint32_t tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+
+    const uint32_t pairs = a.kv_heads * a.blocks;
+    const uint64_t T = tiles_before(a.n_seq, a);
+    if (blockIdx.x == 0 && warp == 0)
+        for (uint32_t s = lane; s < a.n_seq; s += 32u)
+            if (a.len[s] >= a.cap && a.len[s] != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
+    const uint32_t G = sharers(T, a);
+    if (blockIdx.x >= G) return;
+    uint64_t u = blockIdx.x * T / G;
+    const uint64_t u1 = (blockIdx.x + 1ull) * T / G;
+    // The sequence that tile u belongs to, and the tiles before it.
+    uint32_t s = 0;
+    uint64_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32u) {
+        uint64_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) : 0u, incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= (uint32_t)o) incl += up;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + incl * pairs > u);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            s = s0 + at;
+            before += __shfl_sync(0xffffffffu, incl - n, at) * pairs;
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31) * pairs;
+    }
+
+    const uint32_t ring_base = smem_addr(ring) + warp * (STAGES * C::kStage);
+    while (u < u1) {
+        const uint32_t len = tmdev::uniform(a.len[s]), nt = pair_tiles(len, a);
+        if (nt == 0u) {
+            ++s;
+            continue;
+        }
+        const uint32_t start = first_row(len, a.window);
+        const uint32_t pair = (uint32_t)((u - before) / nt), t0 = (uint32_t)((u - before) % nt);
+        const uint32_t tn = (uint32_t)min((uint64_t)(nt - t0), u1 - u);
+        const uint32_t kvh = pair / a.blocks, hb = pair % a.blocks;
+        const uint32_t head0 = kvh * a.group + hb * 8u, heads = min(8u, a.group - hb * 8u);
+        const uint32_t block0 = (start / kTile + t0) * kAttnWarps + warp;  // this warp's first 16 rows; then every 4th
+        const uint32_t *pages = a.table + (size_t)s * a.max_pages;
+        const bool owns_new = t0 + tn == nt;
+
+        // ---- the ring of cached rows ----
+        auto in_sight = [&](uint32_t blk) { return blk * kBlock <= len && blk * kBlock + (kBlock - 1u) >= start; };
+        auto page_of = [&](uint32_t i) {  // of this warp's i-th block
+            const uint32_t blk = block0 + i * kAttnWarps;
+            return i < tn && in_sight(blk) ? pages[blk * kBlock >> a.page_log] : 0u;
+        };
+        auto load = [&](uint32_t i, uint32_t id) {
+            const uint32_t blk = block0 + i * kAttnWarps;
+            if (i < tn && in_sight(blk)) {
+                const bool page = id < a.pages;
+                if (!page && lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+                const size_t row0 = (((size_t)(page ? id : 0u) * a.kv_heads + kvh) << a.page_log) +
+                                    (blk * kBlock & ((1u << a.page_log) - 1u));
+                const uint32_t dst = ring_base + (i % STAGES) * C::kStage;
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    const uint32_t e = c * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), j = blk * kBlock + r;
+                    const bool live = page && j >= start && j < len;  // the rest is zeros; row `len` comes from this call
+                    cp_async16(dst + sw<PITCH>(r, ch), a.kp + (row0 + r) * HD + ch * 8u, live);
+                    cp_async16(dst + C::kPlane + sw<PITCH>(r, ch), a.vp + (row0 + r) * HD + ch * 8u, live);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) load(i, page_of(i));
+        uint32_t next_id = page_of(STAGES - 1);
+
+        // ---- the group's queries, and the new row where this run ends with it: norm, rotation, f16 ----
+        const uint32_t pos = a.pos[s];
+        for (uint32_t x = warp; x < heads + (owns_new ? 1u : 0u); x += kAttnWarps) {
+            const bool is_k = x == heads;
+            const float *src = is_k ? a.k + (size_t)s * a.kv_stride + (size_t)kvh * HD
+                                    : a.q + (size_t)s * a.q_stride + (size_t)(head0 + x) * HD;
+            const float *nw = is_k ? a.k_norm : a.q_norm;
+            float y[EPL], ss = 0.0f;
+#pragma unroll
+            for (int r = 0; r < EPL; ++r) {
+                y[r] = src[lane + 32 * r];
+                ss = fmaf(y[r], y[r], ss);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+            float *row = vec + x * HD;
+#pragma unroll
+            for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = y[r] * inv * nw[lane + 32 * r];
+            __syncwarp();
+            const uint32_t half = a.n_rot / 2u;
+            for (uint32_t i = lane; i < half; i += 32u) {
+                const float angle = (float)pos * a.inv_freq[i], c = cosf(angle), sn = sinf(angle);
+                const float x0 = row[i], x1 = row[i + half];
+                row[i] = x0 * c - x1 * sn;
+                row[i + half] = x0 * sn + x1 * c;
+            }
+            __syncwarp();
+            float top = 0.0f;
+#pragma unroll
+            for (int r = 0; r < EPL; ++r) {
+                y[r] = row[lane + 32 * r];
+                top = fmaxf(top, fabsf(y[r]));
+            }
+            if (is_k) {
+                const uint32_t id = pages[len >> a.page_log];
+                const bool page = id < a.pages;
+                if (!page && lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+                const size_t at = ((((size_t)(page ? id : 0u) * a.kv_heads + kvh) << a.page_log) + (len & ((1u << a.page_log) - 1u))) * HD;
+                const float *vs = a.v + (size_t)s * a.kv_stride + (size_t)kvh * HD;
+#pragma unroll
+                for (int r = 0; r < EPL; ++r) {
+                    const uint32_t e = lane + 32 * r;
+                    const __half hk = __float2half_rn(y[r]), hv = __float2half_rn(vs[e]);
+                    k_new[e] = hk;
+                    v_new[e] = hv;
+                    if (page && hb == 0u) {
+                        a.kp[at + e] = hk;
+                        a.vp[at + e] = hv;
+                    }
+                }
+                continue;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // q = 2^e (hi + lo), |hi| < 2; a vector of zeros, infinities or NaN keeps e = 0
+            int e = (int)((__float_as_uint(top) >> 23) & 0xffu) - 127;
+            e = top > 0.0f && top < INFINITY ? max(-120, min(120, e)) : 0;
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+            for (int r = 0; r < EPL; ++r) {
+                const float z = y[r] * down;
+                const __half hi = __float2half_rn(z);
+                q_hi[x * QP + lane + 32 * r] = hi;
+                q_lo[x * QP + lane + 32 * r] = __float2half_rn(z - __half2float(hi));
+            }
+            if (lane == 0) factor[x] = a.scale_log2e * __uint_as_float((uint32_t)(127 + e) << 23);
+        }
+        for (uint32_t x = heads + warp; x < 8u; x += kAttnWarps) {  // columns of no head
+            for (uint32_t e = lane; e < HD; e += 32u) q_hi[x * QP + e] = q_lo[x * QP + e] = __float2half_rn(0.0f);
+            if (lane == 0) factor[x] = 0.0f;
+        }
+        __syncthreads();
+        uint32_t qh[HD <= 128 ? HD / 16 : 1][2], ql[HD <= 128 ? HD / 16 : 1][2];
+        if (HD <= 128) {
+#pragma unroll
+            for (int kt = 0; kt < (HD <= 128 ? HD / 16 : 1); ++kt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    qh[kt][i] = *(const uint32_t *)(q_hi + g * QP + kt * 16 + i * 8 + 2 * t);
+                    ql[kt][i] = *(const uint32_t *)(q_lo + g * QP + kt * 16 + i * 8 + 2 * t);
+                }
+        }
+        const float f0 = factor[2 * t], f1 = factor[2 * t + 1];
+        float o[HD / 16][4];
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;  // heads 2t and 2t + 1; l: this lane's rows
+
+#pragma unroll 1
+        for (uint32_t i = 0; i < tn; ++i) {
+            const uint32_t blk = block0 + i * kAttnWarps, j0 = blk * kBlock;
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();  // this block has landed for all lanes, and all have read the one before it
+            load(i + STAGES - 1, next_id);
+            next_id = page_of(i + STAGES);
+            if (!in_sight(blk)) continue;
+            const uint32_t kb = ring_base + (i % STAGES) * C::kStage, vb = kb + C::kPlane;
+            if (len - j0 < kBlock) {  // the new row
+                unsigned char *st = ring + (kb - smem_addr(ring));
+                if (lane < HD / 8) {
+                    *(uint4 *)(st + sw<PITCH>(len - j0, lane)) = *(const uint4 *)(k_new + lane * 8);
+                    *(uint4 *)(st + C::kPlane + sw<PITCH>(len - j0, lane)) = *(const uint4 *)(v_new + lane * 8);
+                }
+                __syncwarp();
+            }
+            float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int kt = 0; kt < HD / 16; ++kt) {
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4(kb + sw<PITCH>(lane & 15u, kt * 2 + (lane >> 4)), a0, a1, a2, a3);
+                if (HD <= 128) {
+                    mma_f16(hi, a0, a1, a2, a3, qh[kt % (HD <= 128 ? HD / 16 : 1)][0], qh[kt % (HD <= 128 ? HD / 16 : 1)][1]);
+                    mma_f16(lo, a0, a1, a2, a3, ql[kt % (HD <= 128 ? HD / 16 : 1)][0], ql[kt % (HD <= 128 ? HD / 16 : 1)][1]);
+                } else {
+                    const __half *qp = q_hi + g * QP + kt * 16 + 2 * t;
+                    mma_f16(hi, a0, a1, a2, a3, *(const uint32_t *)qp, *(const uint32_t *)(qp + 8));
+                    qp += 8 * QP;
+                    mma_f16(lo, a0, a1, a2, a3, *(const uint32_t *)qp, *(const uint32_t *)(qp + 8));
+                }
+            }
+            // rows j0 + g and j0 + g + 8, heads 2t and 2t + 1
+            const uint32_t ja = j0 + g, jb = ja + 8u;
+            const bool see_a = ja >= start && ja <= len, see_b = jb >= start && jb <= len;
+            const float s0 = see_a ? (hi[0] + lo[0]) * f0 : -INFINITY, s1 = see_a ? (hi[1] + lo[1]) * f1 : -INFINITY;
+            const float s2 = see_b ? (hi[2] + lo[2]) * f0 : -INFINITY, s3 = see_b ? (hi[3] + lo[3]) * f1 : -INFINITY;
+            if (a.scores) {
+                float *row = a.scores + (((size_t)s * a.kv_heads + kvh) * a.cap + ja) * a.group + hb * 8u + 2 * t;
+                if (see_a && 2 * t < heads) row[0] = s0;
+                if (see_a && 2 * t + 1 < heads) row[1] = s1;
+                row += (size_t)8 * a.group;
+                if (see_b && 2 * t < heads) row[0] = s2;
+                if (see_b && 2 * t + 1 < heads) row[1] = s3;
+            }
+            float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
+#pragma unroll
+            for (int sh = 4; sh < 32; sh <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, sh));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, sh));
+            }
+            x0 = fmaxf(x0, m0);
+            x1 = fmaxf(x1, m1);
+            const float u0 = (x0 == -INFINITY ? 0.0f : x0), u1m = (x1 == -INFINITY ? 0.0f : x1);
+            const float al0 = exp2f(m0 - u0), al1 = exp2f(m1 - u1m);
+            m0 = x0;
+            m1 = x1;
+            const float p0 = exp2f(s0 - u0 + kUnit), p1 = exp2f(s1 - u1m + kUnit);
+            const float p2 = exp2f(s2 - u0 + kUnit), p3 = exp2f(s3 - u1m + kUnit);
+            l0 = fmaf(l0, al0, p0 + p2);
+            l1 = fmaf(l1, al1, p1 + p3);
+            const __half2 pa = __floats2half2_rn(p0, p1), pb = __floats2half2_rn(p2, p3);
+            const float2 fa = __half22float2(pa), fb = __half22float2(pb);
+            const uint32_t h0 = transpose8x8(bits(pa)), h1 = transpose8x8(bits(pb));
+            const uint32_t r0 = transpose8x8(bits(__floats2half2_rn(p0 - fa.x, p1 - fa.y)));
+            const uint32_t r1 = transpose8x8(bits(__floats2half2_rn(p2 - fb.x, p3 - fb.y)));
+            const uint32_t mat = lane >> 3, vr = (lane & 7u) + (mat >> 1) * 8u;
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4_t(vb + sw<PITCH>(vr, mt * 2 + (mat & 1u)), a0, a1, a2, a3);
+                float d[4] = {0, 0, 0, 0};
+                mma_f16(d, a0, a1, a2, a3, h0, h1);
+                mma_f16(d, a0, a1, a2, a3, r0, r1);
+                o[mt][0] = fmaf(o[mt][0], al0, d[0]);
+                o[mt][1] = fmaf(o[mt][1], al1, d[1]);
+                o[mt][2] = fmaf(o[mt][2], al0, d[2]);
+                o[mt][3] = fmaf(o[mt][3], al1, d[3]);
+            }
+        }
+        // ---- the warps' states -> this run's ----
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the ring is free
+        float *wo = (float *)ring;  // [warps][8][HD]
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
+        }
+        if (g == 0) {
+            wm[warp * 8 + 2 * t] = m0;
+            wm[warp * 8 + 2 * t + 1] = m1;
+            wl[warp * 8 + 2 * t] = l0;
+            wl[warp * 8 + 2 * t + 1] = l1;
+        }
+#pragma unroll
+        for (int mt = 0; mt < HD / 16; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                wo[(warp * 8 + 2 * t + (e & 1)) * HD + mt * 16 + g + (e >> 1) * 8] = o[mt][e];
+        __syncthreads();
+        const bool whole = tn == nt;
+        float *part = a.part + ((size_t)blockIdx.x * 2 + (t0 == 0u ? 1 : 0)) * 8 * (HD + 2);
+        for (uint32_t i = tid; i < heads * HD; i += kAttnThreads) {
+            const uint32_t h = i / HD, d = i % HD;
+            float M = wm[h];
+#pragma unroll
+            for (int w = 1; w < kAttnWarps; ++w) M = fmaxf(M, wm[w * 8 + h]);
+            const float top = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float f = exp2f(wm[w * 8 + h] - top);  // a warp that saw no row: 0
+                L = fmaf(f, wl[w * 8 + h], L);
+                O = fmaf(f, wo[(w * 8 + h) * HD + d], O);
+            }
+            if (whole) a.out[((size_t)s * a.heads + head0 + h) * HD + d] = O / L;
+            else part[h * (HD + 2) + 2 + d] = O;
+            if (d == 0) {
+                float *ml = whole ? (a.ml ? a.ml + ((size_t)s * a.heads + head0 + h) * 2 : nullptr) : part + h * (HD + 2);
+                if (ml) {
+                    ml[0] = M;
+                    ml[1] = L;
+                }
+            }
+        }
+        __syncthreads();
+        u += tn;
+        if (u - before == (uint64_t)nt * pairs) {
+            before = u;
+            ++s;
+        }
+    }
+}
+
+// Joins the pieces of pairs that more than one CTA had a run of (grid.z 0), and counts the attention of 1024 rows a CTA
+// (grid.z from 1 on).
+constexpr uint32_t kJoinThreads = 256, kCountRows = 1024;
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(const paged_args a) {
+    __shared__ float sm[32], sl[32];
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    const uint32_t s = blockIdx.y, tid = threadIdx.x, len = a.len[s], nt = pair_tiles(len, a);
+    if (nt == 0u) return;
+    const uint64_t T = tiles_before(a.n_seq, a), before = tiles_before(s, a);
+    const uint32_t G = sharers(T, a);
+    const size_t stride = 8 * (HD + 2);
+    // Partial result c of a pair whose first tile is u: CTA i0 has begun it, the others carry on.
+    auto piece = [&](uint32_t i0, uint32_t i) { return a.part + ((size_t)i * 2 + (i == i0 ? 1 : 0)) * stride; };
+    if (blockIdx.z == 0) {
+        const uint32_t pair = blockIdx.x, kvh = pair / a.blocks, hb = pair % a.blocks;
+        const uint32_t head0 = kvh * a.group + hb * 8u, heads = min(8u, a.group - hb * 8u);
+        const uint64_t u = before + (uint64_t)pair * nt;
+        const uint32_t i0 = cta_of(u, T, G), i1 = cta_of(u + nt - 1, T, G);
+        if (i0 == i1) return;
+        for (uint32_t e = tid; e < heads * HD; e += kJoinThreads) {
+            const uint32_t h = e / HD, d = e % HD;
+            float M = -INFINITY, L = 0.0f, O = 0.0f;
+            for (uint32_t c0 = i0; c0 <= i1; c0 += 8) {
+                float mb[8], lb[8], ob[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float *p = piece(i0, min(c0 + c, i1)) + h * (HD + 2);
+                    mb[c] = c0 + c <= i1 ? p[0] : -INFINITY;
+                    lb[c] = p[1];
+                    ob[c] = p[2 + d];
+                }
+                float top = M;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) top = fmaxf(top, mb[c]);
+                const float use = top == -INFINITY ? 0.0f : top, al = exp2f(M - use);
+                L *= al;
+                O *= al;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (c0 + c > i1) break;
+                    const float f = exp2f(mb[c] - use);
+                    L = fmaf(f, lb[c], L);
+                    O = fmaf(f, ob[c], O);
+                }
+                M = top;
+            }
+            a.out[((size_t)s * a.heads + head0 + h) * HD + d] = O / L;
+        }
+        return;
+    }
+    const uint32_t row0 = (blockIdx.z - 1u) * kCountRows;
+    if (blockIdx.x % a.blocks != 0u || row0 > len) return;
+    const uint32_t kvh = blockIdx.x / a.blocks;
+    if (tid < a.group) {
+        const uint32_t hb = tid / 8u, h = tid % 8u;
+        const uint64_t u = before + (uint64_t)(kvh * a.blocks + hb) * nt;
+        const uint32_t i0 = cta_of(u, T, G), i1 = cta_of(u + nt - 1, T, G);
+        float M = -INFINITY, L = 0.0f;
+        if (i0 == i1) {
+            const float *ml = a.ml + ((size_t)s * a.heads + kvh * a.group + tid) * 2;
+            M = ml[0];
+            L = ml[1];
+        } else {
+            for (uint32_t i = i0; i <= i1; ++i) M = fmaxf(M, piece(i0, i)[h * (HD + 2)]);
+            const float use = M == -INFINITY ? 0.0f : M;
+            for (uint32_t i = i0; i <= i1; ++i) {
+                const float *p = piece(i0, i) + h * (HD + 2);
+                L = fmaf(exp2f(p[0] - use), p[1], L);
+            }
+        }
+        sm[tid] = M - kUnit;
+        sl[tid] = L;
+    }
+    __syncthreads();
+    const uint32_t start = first_row(len, a.window);
+    const size_t base = ((size_t)s * a.kv_heads + kvh) * a.cap;
+    for (uint32_t j = row0 + tid; j < row0 + kCountRows && j <= len; j += kJoinThreads) {
+        float w = a.w_in && j < len ? a.w_in[base + j] : 0.0f;  // the new row has drawn nothing before
+        if (j >= start) {
+            float sum = 0.0f;
+            for (uint32_t h = 0; h < a.group; ++h) sum += exp2f(a.scores[(base + j) * a.group + h] - sm[h]) / sl[h];
+            w += sum;
+        }
+        a.w_out[base + j] = w;
+    }
+}
+
+template <int HD>
+cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a, uint64_t &kernels) {
+    using C = attn_cfg<HD>;
+    static std::atomic<bool> attr_done[64] = {};  // per device; contexts of a process share it
+    const int device = ctx->device;
+    if (device < 0 || device >= 64 || !attr_done[device].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(attention_paged_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kBytes);
+        if (e != cudaSuccess) return e;
+        if (device >= 0 && device < 64) attr_done[device].store(true, std::memory_order_release);
+    }
+    const uint64_t tiles = ((uint64_t)a.cap + kTile - 1) / kTile, pairs = (uint64_t)a.n_seq * a.kv_heads * a.blocks;
+    const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), kMostCtas);
+    a.ctas = (uint32_t)(pairs * tiles < places ? pairs * tiles : places);
+    cudaError_t e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
+    kernels = 1;
+    if (e == cudaSuccess && (tiles > 1 || a.w_out)) {  // (pairs of one tile are never cut)
+        const uint32_t z = a.w_out ? 1u + (a.cap + kCountRows - 1) / kCountRows : 1u;
+        e = tm_launch_pdl(ctx, attention_paged_join_kernel<HD>, dim3(a.kv_heads * a.blocks, a.n_seq, z), dim3(kJoinThreads), 0, a);
+        kernels = 2;
+    }
+    return e;
+}
+
+// ---- copies between dense planes and pages ---------------------------------------------------------
+//
+// Moves 4 head_dim bytes a row and KV head each way and computes nothing: 16 bytes a thread and load, all loads of a
+// thread before its first store.  A CTA takes up to 64 rows of one run, one head, keys or values.
+constexpr uint32_t kCopyRows = 64, kCopyThreads = 256;
+struct copy_runs {
+    uint32_t n;
+    uint32_t tile0[TM_CUDA_PREFILL_SEGMENTS + 1];
+    uint32_t seq[TM_CUDA_PREFILL_SEGMENTS], at[TM_CUDA_PREFILL_SEGMENTS], row0[TM_CUDA_PREFILL_SEGMENTS], rows[TM_CUDA_PREFILL_SEGMENTS];
+};
+struct copy_args {
+    __half *kc, *vc, *kp, *vp;
+    const uint32_t *table;
+    uint32_t *status;
+    uint32_t pages, page_log, max_pages, kv_heads, cap;
+};
+
+template <int HD, bool TO_PAGES>
+__global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const copy_args a, const __grid_constant__ copy_runs runs) {
+    constexpr uint32_t kChunks = HD / 8, kEach = kCopyRows * kChunks / kCopyThreads;  // 16-byte chunks of a row; a thread's
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    uint32_t r = 0;
+    while (r + 1u < runs.n && runs.tile0[r + 1u] <= blockIdx.x) ++r;
+    const uint32_t first = (blockIdx.x - runs.tile0[r]) * kCopyRows, rows = min(kCopyRows, runs.rows[r] - first);
+    const uint32_t row0 = runs.row0[r] + first, h = blockIdx.y;
+    __half *dense = (blockIdx.z ? a.vc : a.kc) + (((size_t)runs.seq[r] * a.kv_heads + h) * a.cap + row0) * HD;
+    __half *pool = blockIdx.z ? a.vp : a.kp;
+    const uint32_t *pages = a.table + (size_t)runs.at[r] * a.max_pages;
+    uint4 v[kEach];
+    __half *to[kEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t e = i * kCopyThreads + threadIdx.x, row = e / kChunks, ch = e % kChunks;
+        to[i] = nullptr;
+        if (row >= rows) continue;
+        const uint32_t j = row0 + row, id = pages[j >> a.page_log];
+        const bool page = id < a.pages;
+        if (!page) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+        __half *in = dense + (size_t)row * HD + ch * 8u;
+        __half *paged = pool + ((((size_t)(page ? id : 0u) * a.kv_heads + h) << a.page_log) + (j & ((1u << a.page_log) - 1u))) * HD + ch * 8u;
+        if (TO_PAGES) {
+            v[i] = *(const uint4 *)in;
+            to[i] = page ? paged : nullptr;
+        } else {
+            v[i] = page ? *(const uint4 *)paged : make_uint4(0u, 0u, 0u, 0u);
+            to[i] = in;
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i)
+        if (to[i]) *(uint4 *)to[i] = v[i];
+}
+
+// ---- eviction --------------------------------------------------------------------------------------
+//
+// Per (sequence, KV head): the first `first` rows, the last `recent` rows, and of those between the ones with the largest
+// weights, `keep` in all, in their order.  One CTA finds the smallest weight that stays by three counting passes over
+// 11, 11 and 10 bits of the weights' order-preserving integers (1024 threads, the weights come from L2 after the first),
+// then writes the list of rows; a second launch moves the rows.  What bounds it: the rows' bytes, 8 head_dim each.
+constexpr uint32_t kEvictThreads = 1024;
+
+struct evict_args {
+    __half *kp, *vp;
+    const uint32_t *table, *to, *len;
+    uint32_t *len_out;  // none where it is `len` itself, which the second launch still reads
+    const float *w;
+    float *w_out;
+    uint32_t *kept, *status;
+    uint32_t kv_heads, pages, page_log, max_pages, cap, keep, first, recent;
+};
+
+// Weights in order: NaN below everything, -0 as +0.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (isnan(w)) return 0u;
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// Exclusive prefix sum over the CTA's threads, and the total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warps, uint32_t &total) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    uint32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31u) warps[warp] = incl;
+    __syncthreads();
+    uint32_t w = warps[lane], sum = w;  // 32 warps
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= (uint32_t)o) sum += up;
+    }
+    total = __shfl_sync(0xffffffffu, sum, 31);
+    return __shfl_sync(0xffffffffu, sum - w, warp) + incl - v;
+}
+
+__global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const evict_args a) {
+    __shared__ uint32_t hist[2048], warps[32], found[2];
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    const uint32_t s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, len = a.len[s];
+    if (len == kSeqNone || len > a.cap) {
+        if (h == 0 && tid == 0) {
+            if (len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
+            if (a.len_out) a.len_out[s] = len;
+        }
+        return;
+    }
+    if (a.len_out && h == 0 && tid == 0) a.len_out[s] = min(len, a.keep);
+    const size_t head = (size_t)s * a.kv_heads + h;
+    const float *w = a.w + head * a.cap;
+    uint32_t *kept = a.kept + head * a.keep;
+    const uint32_t n = min(len, a.keep);
+    if (len <= a.keep) {
+        for (uint32_t i = tid; i < a.keep; i += kEvictThreads) kept[i] = i < len ? i : TM_CUDA_SEQ_NONE;
+    } else {
+        const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
+        // The want-th largest key between lo and hi, digit by digit: `prefix` its bits so far, `left` how many are
+        // still wanted among the keys that begin with them.
+        uint32_t prefix = 0u, left = want;
+        const uint32_t shift[3] = {21u, 10u, 0u}, width[3] = {11u, 11u, 10u};
+        if (want > 0u) {
+#pragma unroll 1
+            for (int p = 0; p < 3; ++p) {
+                for (uint32_t b = tid; b < 2048u; b += kEvictThreads) hist[b] = 0u;
+                __syncthreads();
+                const uint32_t mask = p == 0 ? 0u : ~0u << (shift[p] + width[p]);
+                for (uint32_t j = lo + tid; j < hi; j += kEvictThreads) {
+                    const uint32_t key = weight_key(w[j]);
+                    if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift[p]) & ((1u << width[p]) - 1u)], 1u);
+                }
+                __syncthreads();
+                // Thread i: bins 2047 - 2i and below it, so that a prefix sum counts from the top.
+                const uint32_t b1 = 2047u - 2u * tid, c1 = hist[b1], c0 = hist[b1 - 1u];
+                uint32_t total;
+                const uint32_t above = block_scan(c1 + c0, warps, total);
+                if (above < left && above + c1 + c0 >= left) {
+                    const bool upper = above + c1 >= left;
+                    found[0] = upper ? b1 : b1 - 1u;
+                    found[1] = left - above - (upper ? 0u : c1);
+                }
+                __syncthreads();
+                prefix |= found[0] << shift[p];
+                left = found[1];
+                __syncthreads();
+            }
+        }
+        // Each thread lists a contiguous strip of rows: keys above the border, and the first `left` equal to it.
+        const uint32_t strip = (len + kEvictThreads - 1u) / kEvictThreads, j0 = min(len, tid * strip), j1 = min(len, j0 + strip);
+        uint32_t equal = 0u, total;
+        if (want > 0u)
+            for (uint32_t j = max(j0, lo); j < min(j1, hi); ++j) equal += weight_key(w[j]) == prefix ? 1u : 0u;
+        uint32_t eq = block_scan(equal, warps, total);
+        auto stays = [&](uint32_t j, uint32_t &e) {
+            if (j < lo || j >= hi) return true;
+            if (want == 0u) return false;
+            const uint32_t key = weight_key(w[j]);
+            return key > prefix || (key == prefix && e++ < left);
+        };
+        uint32_t mine = 0u, e = eq;
+        for (uint32_t j = j0; j < j1; ++j) mine += stays(j, e) ? 1u : 0u;
+        uint32_t at = block_scan(mine, warps, total);
+        e = eq;
+        for (uint32_t j = j0; j < j1; ++j)
+            if (stays(j, e)) kept[at++] = j;
+    }
+    __syncthreads();
+    // The weights go with their rows.  A row never moves up, so reading a stretch before it is written is enough in place.
+    float *w_out = a.w_out + head * a.cap;
+    for (uint32_t i0 = 0; i0 < n; i0 += kEvictThreads) {
+        const uint32_t i = i0 + tid;
+        const float v = i < n ? w[kept[i]] : 0.0f;
+        __syncthreads();
+        if (i < n) w_out[i] = v;
+        __syncthreads();
+    }
+}
+
+// Moves the kept rows.  In place a CTA takes 64 bytes of every row of a head, so that the columns need not wait for one
+// another, and goes up the rows: what it stores lies at or below what it has read.  Into other pages every stretch of rows
+// is a CTA of its own.
+constexpr uint32_t kMoveThreads = 256, kMoveEach = 8;
+template <int HD, bool IN_PLACE>
+__global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const evict_args a) {
+    constexpr uint32_t kLanes = IN_PLACE ? 4 : HD / 8, kSlices = HD / 8 / kLanes, kRows = kMoveThreads / kLanes * kMoveEach;
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    const uint32_t s = blockIdx.y / a.kv_heads, h = blockIdx.y % a.kv_heads, len = a.len[s];
+    if (len > a.cap || (IN_PLACE && len <= a.keep)) return;
+    const uint32_t n = min(len, a.keep);
+    const uint32_t slice = blockIdx.x % kSlices, is_v = blockIdx.x / kSlices % 2u, tile = blockIdx.x / (2u * kSlices);
+    __half *pool = is_v ? a.vp : a.kp;
+    const uint32_t *from = a.table + (size_t)s * a.max_pages, *to = a.to + (size_t)s * a.max_pages;
+    const uint32_t *kept = a.kept + (size_t)blockIdx.y * a.keep;
+    const uint32_t low = (1u << a.page_log) - 1u, lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, col = (slice * kLanes + lane) * 8u;
+    auto place = [&](const uint32_t *pages, uint32_t j) -> __half * {
+        const uint32_t id = pages[j >> a.page_log];
+        if (id >= a.pages) {
+            atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+            return nullptr;
+        }
+        return pool + ((((size_t)id * a.kv_heads + h) << a.page_log) + (j & low)) * HD + col;
+    };
+    for (uint32_t i0 = tile * kRows; i0 < n; i0 += IN_PLACE ? kRows : n) {
+        uint4 v[kMoveEach];
+        __half *dst[kMoveEach];
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) {
+            const uint32_t i = i0 + x * (kMoveThreads / kLanes) + r;
+            dst[x] = nullptr;
+            if (i >= n) continue;
+            const __half *src = place(from, kept[i]);
+            dst[x] = place(to, i);
+            v[x] = src ? *(const uint4 *)src : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (IN_PLACE) __syncthreads();  // the whole stretch is read
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x)
+            if (dst[x]) *(uint4 *)dst[x] = v[x];
+        if (IN_PLACE) __syncthreads();  // and written before the next is read
+    }
+}
+// The lengths, where they replace the ones that both launches above read.
+__global__ void kv_evict_lengths_kernel(uint32_t *len, uint32_t n_seq, uint32_t keep, uint32_t cap) {
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    const uint32_t s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s < n_seq && len[s] <= cap) len[s] = min(len[s], keep);
+}
+
+template <int HD>
+cudaError_t launch_move(tm_cuda_ctx *ctx, const evict_args &a, uint32_t n_seq, bool in_place) {
+    const uint32_t rows = kMoveThreads / (HD / 8) * kMoveEach, most = a.keep < a.cap ? a.keep : a.cap;
+    if (in_place)
+        return tm_launch_pdl(ctx, kv_evict_move_kernel<HD, true>, dim3(2 * (HD / 32), n_seq * a.kv_heads), dim3(kMoveThreads), 0, a);
+    return tm_launch_pdl(ctx, kv_evict_move_kernel<HD, false>, dim3(2 * ((most + rows - 1) / rows), n_seq * a.kv_heads),
+                         dim3(kMoveThreads), 0, a);
+}
+
+template <int HD>
+cudaError_t launch_copy(tm_cuda_ctx *ctx, const copy_args &a, const copy_runs &runs, bool to_pages) {
+    const dim3 grid(runs.tile0[runs.n], a.kv_heads, 2);
+    return to_pages ? tm_launch_pdl(ctx, kv_pages_copy_kernel<HD, true>, grid, dim3(kCopyThreads), 0, a, runs)
+                    : tm_launch_pdl(ctx, kv_pages_copy_kernel<HD, false>, grid, dim3(kCopyThreads), 0, a, runs);
+}
+
+struct pool_shape {
+    uint32_t pages, page_rows, max_pages, kv_heads, head_dim;
+};
+int check_pool(const pool_shape &p, const char *what, char *err, size_t err_cap) {
+    if (!pages_ok(p.head_dim, p.page_rows) || p.kv_heads == 0 || p.kv_heads > 4096u || p.pages == 0 || p.max_pages == 0 ||
+        (uint64_t)p.max_pages * p.page_rows > 1u << 25 || (uint64_t)p.pages * p.kv_heads * p.page_rows > 0xffffffffu)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS,
+                       "%s: head_dim %u (32, 64, 128 or 256), %u KV heads, %u pages of %u rows (16, 32, 64, 128 or 256), %u "
+                       "pages a sequence", what, p.head_dim, p.kv_heads, p.pages, p.page_rows, p.max_pages);
+    return TM_CUDA_OK;
+}
+size_t pool_bytes(const pool_shape &p) { return (size_t)p.pages * p.kv_heads * p.page_rows * p.head_dim * 2; }
+
+}  // namespace
+
+extern "C" {
+
+int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows) { return pages_ok(head_dim, page_rows) ? 1 : 0; }
+
+// Partial results of CTAs' runs; then, where attention is counted, (max, sum) of every head and the scores of every row.
+size_t tm_cuda_attention_paged_scratch_bytes(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                             uint32_t page_rows, uint32_t max_pages, int weights) {
+    (void)kv_heads;
+    const size_t part = (size_t)kMostCtas * 2 * 8 * (head_dim + 2) * 4;
+    return weights ? part + (size_t)n_seq * heads * 4 * (2 + (size_t)max_pages * page_rows) : part;
+}
+
+int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_cuda_buffer *k, tm_cuda_buffer *v,
+                                       tm_cuda_buffer *q_norm, tm_cuda_buffer *k_norm, tm_cuda_buffer *inv_freq,
+                                       tm_cuda_buffer *k_pages, tm_cuda_buffer *v_pages, tm_cuda_buffer *table,
+                                       tm_cuda_buffer *out, tm_cuda_buffer *scratch, tm_cuda_buffer *pos_buf,
+                                       tm_cuda_buffer *len_buf, tm_cuda_buffer *status, tm_cuda_buffer *weights_in,
+                                       tm_cuda_buffer *weights_out, uint32_t n_seq, uint32_t q_stride, uint32_t kv_stride,
+                                       uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t n_rot,
+                                       uint32_t pages, uint32_t page_rows, uint32_t max_pages, uint32_t window, float eps,
+                                       float scale, char *err, size_t err_cap) {
+    TM_ENTER();
+    const pool_shape shape = {pages, page_rows, max_pages, kv_heads, head_dim};
+    if (const int rc = check_pool(shape, "paged attention", err, err_cap)) return rc;
+    if (heads == 0 || heads % kv_heads != 0 || heads / kv_heads > 32u || n_rot == 0 || n_rot > head_dim || n_rot % 2 != 0)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "paged attention: heads %u/%u (1 to 32 a KV head), n_rot %u of head_dim %u",
+                       heads, kv_heads, n_rot, head_dim);
+    if (n_seq == 0 || n_seq > TM_CUDA_PAGED_MAX_SEQUENCES)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "sequence count %u outside 1..%u", n_seq, (unsigned)TM_CUDA_PAGED_MAX_SEQUENCES);
+    if (weights_in && !weights_out)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "attention weights are given but not asked for");
+    if (q_stride == 0) q_stride = heads * head_dim;
+    if (kv_stride == 0) kv_stride = kv_heads * head_dim;
+    if (q_stride < heads * head_dim || kv_stride < kv_heads * head_dim)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "row strides %u / %u below the row widths", q_stride, kv_stride);
+    const size_t nq = ((size_t)(n_seq - 1) * q_stride + (size_t)heads * head_dim) * 4;
+    const size_t nkv = ((size_t)(n_seq - 1) * kv_stride + (size_t)kv_heads * head_dim) * 4;
+    const size_t cap = (size_t)max_pages * page_rows, nout = (size_t)n_seq * heads * head_dim * 4;
+    const size_t nw = (size_t)n_seq * kv_heads * cap * 4, ntable = (size_t)n_seq * max_pages * 4;
+    const size_t nscratch = tm_cuda_attention_paged_scratch_bytes(n_seq, heads, kv_heads, head_dim, page_rows, max_pages, weights_out != nullptr);
+    TM_CHECK_IN(q, nq, "q");
+    TM_CHECK_IN(k, nkv, "k");
+    TM_CHECK_IN(v, nkv, "v");
+    TM_CHECK_IN(q_norm, (size_t)head_dim * 4, "q norm");
+    TM_CHECK_IN(k_norm, (size_t)head_dim * 4, "k norm");
+    TM_CHECK_IN(inv_freq, (size_t)(n_rot / 2) * 4, "inv_freq");
+    TM_CHECK_BUF(k_pages, pool_bytes(shape), "K pages");
+    TM_CHECK_BUF(v_pages, pool_bytes(shape), "V pages");
+    TM_CHECK_IN(table, ntable, "page table");
+    TM_CHECK_BUF(out, nout, "attention output");
+    TM_CHECK_BUF(scratch, nscratch, "paged attention scratch");
+    TM_CHECK_IN(pos_buf, (size_t)n_seq * 4, "positions");
+    TM_CHECK_IN(len_buf, (size_t)n_seq * 4, "lengths");
+    TM_CHECK_BUF(status, 4, "status");
+    if (weights_in) TM_CHECK_IN(weights_in, nw, "attention weights");
+    if (weights_out) TM_CHECK_BUF(weights_out, nw, "attention weights");
+    const tm_span spans[] = {{k_pages, pool_bytes(shape), true, "K pages"}, {v_pages, pool_bytes(shape), true, "V pages"},
+                             {out, nout, true, "attention output"}, {scratch, nscratch, true, "scratch"}, {status, 4, true, "status"},
+                             {weights_out, nw, true, "attention weights"}, {weights_in, nw, false, "attention weights"},
+                             {q, nq, false, "q"}, {k, nkv, false, "k"}, {v, nkv, false, "v"},
+                             {q_norm, (size_t)head_dim * 4, false, "q norm"}, {k_norm, (size_t)head_dim * 4, false, "k norm"},
+                             {inv_freq, (size_t)(n_rot / 2) * 4, false, "inv_freq"}, {table, ntable, false, "page table"},
+                             {pos_buf, (size_t)n_seq * 4, false, "positions"}, {len_buf, (size_t)n_seq * 4, false, "lengths"}};
+    if (const int rc = tm_check_disjoint(spans, sizeof spans / sizeof *spans, 5, 6, err, err_cap)) return rc;
+    paged_args a = {};
+    a.q = (const float *)q->dev;
+    a.k = (const float *)k->dev;
+    a.v = (const float *)v->dev;
+    a.q_norm = (const float *)q_norm->dev;
+    a.k_norm = (const float *)k_norm->dev;
+    a.inv_freq = (const float *)inv_freq->dev;
+    a.kp = (__half *)k_pages->dev;
+    a.vp = (__half *)v_pages->dev;
+    a.table = (const uint32_t *)table->dev;
+    a.pos = (const uint32_t *)pos_buf->dev;
+    a.len = (const uint32_t *)len_buf->dev;
+    a.out = (float *)out->dev;
+    a.part = (float *)scratch->dev;
+    if (weights_out) {
+        a.ml = a.part + (size_t)kMostCtas * 2 * 8 * (head_dim + 2);
+        a.scores = a.ml + (size_t)n_seq * heads * 2;
+        a.w_in = weights_in ? (const float *)weights_in->dev : nullptr;
+        a.w_out = (float *)weights_out->dev;
+    }
+    a.status = (uint32_t *)status->dev;
+    a.n_seq = n_seq;
+    a.q_stride = q_stride;
+    a.kv_stride = kv_stride;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.group = heads / kv_heads;
+    a.blocks = (a.group + 7u) / 8u;
+    a.n_rot = n_rot;
+    a.pages = pages;
+    a.page_log = log2_of(page_rows);
+    a.max_pages = max_pages;
+    a.cap = (uint32_t)cap;
+    a.window = window;
+    a.eps = eps;
+    a.scale_log2e = scale * 1.4426950408889634f;
+    TM_OP_BEGIN("attention_decode_paged");
+    uint64_t kernels = 0;
+    TM_CUDA_TRY(head_dim == 32    ? launch_paged<32>(ctx, a, kernels)
+                : head_dim == 64  ? launch_paged<64>(ctx, a, kernels)
+                : head_dim == 128 ? launch_paged<128>(ctx, a, kernels)
+                                  : launch_paged<256>(ctx, a, kernels));
+    TM_OP_END(kernels);
+}
+
+int tm_cuda_kv_pages_copy_f16(tm_cuda_ctx *ctx, tm_cuda_buffer *k_cache, tm_cuda_buffer *v_cache, tm_cuda_buffer *k_pages,
+                              tm_cuda_buffer *v_pages, tm_cuda_buffer *table, tm_cuda_buffer *status, uint32_t pages,
+                              uint32_t page_rows, uint32_t max_pages, uint32_t kv_heads, uint32_t head_dim, uint32_t cap,
+                              int to_pages, uint32_t n_runs, const uint32_t *runs, char *err, size_t err_cap) {
+    TM_ENTER();
+    const pool_shape shape = {pages, page_rows, max_pages, kv_heads, head_dim};
+    if (const int rc = check_pool(shape, "page copy", err, err_cap)) return rc;
+    if (cap == 0 || n_runs == 0 || n_runs > TM_CUDA_PREFILL_SEGMENTS || !runs)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "page copy: capacity %u, %u runs (1 .. %u)", cap, n_runs,
+                       (unsigned)TM_CUDA_PREFILL_SEGMENTS);
+    copy_runs r;
+    r.n = n_runs;
+    uint32_t seqs = 0, tables = 0;
+    uint64_t tiles = 0;
+    for (uint32_t i = 0; i < n_runs; ++i) {
+        const uint32_t *p = runs + 4 * (size_t)i;
+        if (p[3] == 0 || (uint64_t)p[2] + p[3] > cap || (uint64_t)p[2] + p[3] > (uint64_t)max_pages * page_rows ||
+            p[0] > 0xfffffffeu || p[1] > 0xfffffffeu)
+            return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "run %u: rows %u..%llu of capacity %u, pages of %llu", i, p[2],
+                           (unsigned long long)p[2] + p[3], cap, (unsigned long long)max_pages * page_rows);
+        for (uint32_t j = 0; j < i; ++j) {  // two runs store the same row
+            const uint32_t *o = runs + 4 * (size_t)j, of = to_pages ? 1 : 0;
+            if (o[of] == p[of] && o[2] < p[2] + p[3] && p[2] < o[2] + o[3])
+                return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "runs %u and %u store the same rows", j, i);
+        }
+        r.tile0[i] = (uint32_t)tiles;
+        r.seq[i] = p[0];
+        r.at[i] = p[1];
+        r.row0[i] = p[2];
+        r.rows[i] = p[3];
+        tiles += (p[3] + kCopyRows - 1) / kCopyRows;
+        if (p[0] >= seqs) seqs = p[0] + 1u;
+        if (p[1] >= tables) tables = p[1] + 1u;
+    }
+    if (tiles > 0x7fffffffu) return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "page copy: %llu tiles", (unsigned long long)tiles);
+    for (uint32_t i = n_runs; i <= TM_CUDA_PREFILL_SEGMENTS; ++i) r.tile0[i] = (uint32_t)tiles;
+    // (128-bit product: sequence numbers are the caller's)
+    const unsigned __int128 want = (unsigned __int128)seqs * kv_heads * cap * head_dim * 2;
+    if (want > ((unsigned __int128)1 << 62)) return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "page copy: %u dense sequences", seqs);
+    const size_t ndense = (size_t)want, ntable = (size_t)tables * max_pages * 4;
+    tm_cuda_buffer *const wk = to_pages ? k_pages : k_cache, *const wv = to_pages ? v_pages : v_cache;
+    tm_cuda_buffer *const rk = to_pages ? k_cache : k_pages, *const rv = to_pages ? v_cache : v_pages;
+    const size_t nw = to_pages ? pool_bytes(shape) : ndense, nr = to_pages ? ndense : pool_bytes(shape);
+    TM_CHECK_BUF(wk, nw, to_pages ? "K pages" : "K cache");
+    TM_CHECK_BUF(wv, nw, to_pages ? "V pages" : "V cache");
+    TM_CHECK_IN(rk, nr, to_pages ? "K cache" : "K pages");
+    TM_CHECK_IN(rv, nr, to_pages ? "V cache" : "V pages");
+    TM_CHECK_IN(table, ntable, "page table");
+    TM_CHECK_BUF(status, 4, "status");
+    const tm_span spans[] = {{wk, nw, true, "keys"}, {wv, nw, true, "values"}, {status, 4, true, "status"},
+                             {rk, nr, false, "keys"}, {rv, nr, false, "values"}, {table, ntable, false, "page table"}};
+    if (const int rc = tm_check_disjoint(spans, sizeof spans / sizeof *spans, 0, 0, err, err_cap)) return rc;
+    const copy_args a = {(__half *)k_cache->dev, (__half *)v_cache->dev, (__half *)k_pages->dev, (__half *)v_pages->dev,
+                         (const uint32_t *)table->dev, (uint32_t *)status->dev, pages, log2_of(page_rows), max_pages,
+                         kv_heads, cap};
+    TM_OP_BEGIN("kv_pages_copy");
+    TM_CUDA_TRY(head_dim == 32    ? launch_copy<32>(ctx, a, r, to_pages)
+                : head_dim == 64  ? launch_copy<64>(ctx, a, r, to_pages)
+                : head_dim == 128 ? launch_copy<128>(ctx, a, r, to_pages)
+                                  : launch_copy<256>(ctx, a, r, to_pages));
+    TM_OP_END(1);
+}
+
+int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_buffer *v_pages, tm_cuda_buffer *table,
+                           tm_cuda_buffer *to_table, tm_cuda_buffer *len_buf, tm_cuda_buffer *len_out,
+                           tm_cuda_buffer *weights, tm_cuda_buffer *weights_out, tm_cuda_buffer *kept,
+                           tm_cuda_buffer *status, uint32_t n_seq, uint32_t kv_heads, uint32_t head_dim, uint32_t pages,
+                           uint32_t page_rows, uint32_t max_pages, uint32_t keep, uint32_t first, uint32_t recent, char *err,
+                           size_t err_cap) {
+    TM_ENTER();
+    const pool_shape shape = {pages, page_rows, max_pages, kv_heads, head_dim};
+    if (const int rc = check_pool(shape, "eviction", err, err_cap)) return rc;
+    const size_t cap = (size_t)max_pages * page_rows;
+    if (n_seq == 0 || (uint64_t)n_seq * kv_heads > 65535u)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: %u sequences of %u KV heads (at most 65535 together)", n_seq, kv_heads);
+    if (keep == 0 || keep > cap || (uint64_t)first + recent > keep)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: keep %u of at most %zu rows, the first %u and the last %u among them",
+                       keep, cap, first, recent);
+    const size_t nw = (size_t)n_seq * kv_heads * cap * 4, nk = (size_t)n_seq * kv_heads * keep * 4;
+    const size_t ntable = (size_t)n_seq * max_pages * 4, nlen = (size_t)n_seq * 4;
+    TM_CHECK_BUF(k_pages, pool_bytes(shape), "K pages");
+    TM_CHECK_BUF(v_pages, pool_bytes(shape), "V pages");
+    TM_CHECK_IN(table, ntable, "page table");
+    TM_CHECK_IN(to_table, ntable, "page table to move to");
+    TM_CHECK_IN(len_buf, nlen, "lengths");
+    TM_CHECK_BUF(len_out, nlen, "new lengths");
+    TM_CHECK_IN(weights, nw, "attention weights");
+    TM_CHECK_BUF(weights_out, nw, "kept rows' weights");
+    TM_CHECK_BUF(kept, nk, "kept rows");
+    TM_CHECK_BUF(status, 4, "status");
+    const bool same_len = len_out->dev == len_buf->dev;
+    const tm_span spans[] = {{k_pages, pool_bytes(shape), true, "K pages"}, {v_pages, pool_bytes(shape), true, "V pages"},
+                             {weights_out, nw, true, "kept rows' weights"}, {weights, nw, false, "attention weights"},
+                             {kept, nk, true, "kept rows"}, {status, 4, true, "status"}, {table, ntable, false, "page table"},
+                             {to_table, ntable, false, "page table to move to"}, {len_out, nlen, true, "new lengths"},
+                             {same_len ? nullptr : len_buf, nlen, false, "lengths"}};
+    if (const int rc = tm_check_disjoint(spans, sizeof spans / sizeof *spans, 2, 3, err, err_cap)) return rc;
+    const bool in_place = to_table->dev == table->dev;
+    const evict_args a = {(__half *)k_pages->dev, (__half *)v_pages->dev, (const uint32_t *)table->dev,
+                          (const uint32_t *)to_table->dev, (const uint32_t *)len_buf->dev,
+                          same_len ? nullptr : (uint32_t *)len_out->dev, (const float *)weights->dev, (float *)weights_out->dev,
+                          (uint32_t *)kept->dev, (uint32_t *)status->dev, kv_heads, pages, log2_of(page_rows), max_pages,
+                          (uint32_t)cap, keep, first, recent};
+    TM_OP_BEGIN("kv_pages_evict");
+    TM_CUDA_TRY(tm_launch_pdl(ctx, kv_evict_select_kernel, dim3(kv_heads, n_seq), dim3(kEvictThreads), 0, a));
+    TM_CUDA_TRY(head_dim == 32    ? launch_move<32>(ctx, a, n_seq, in_place)
+                : head_dim == 64  ? launch_move<64>(ctx, a, n_seq, in_place)
+                : head_dim == 128 ? launch_move<128>(ctx, a, n_seq, in_place)
+                                  : launch_move<256>(ctx, a, n_seq, in_place));
+    if (same_len)
+        TM_CUDA_TRY(tm_launch_pdl(ctx, kv_evict_lengths_kernel, dim3((n_seq + 127) / 128), dim3(128), 0, (uint32_t *)len_out->dev,
+                                  n_seq, keep, (uint32_t)cap));
+    TM_OP_END(same_len ? 3 : 2);
+}
+
+}  // extern "C"

@@ -23,7 +23,10 @@ GEMM_MAX_BATCH = 32
 GEMM_MMA_MAX_BATCH = 8192
 PRO_NONE, PRO_RMSNORM, PRO_SILU_MUL, PRO_GELU_MUL, PRO_F16 = 0, 1, 2, 3, 4
 EPI_STORE, EPI_ADD, EPI_SILU_MUL_F16, EPI_GELU_MUL_F16 = 0, 1, 2, 3
-STATUS_PAST_CAPACITY, STATUS_LATE = 1, 2
+STATUS_PAST_CAPACITY, STATUS_LATE, STATUS_BAD_PAGE = 1, 2, 4
+SEQ_NONE = 0xFFFFFFFF
+PAGED_MAX_SEQUENCES = 1024
+LOGITS_MAX, LOGITS_PARTIAL_BYTES = 1 << 21, 2048
 
 
 class CudaError(RuntimeError):
@@ -79,6 +82,10 @@ _OPS = {
     "rows_indirect_seq_f32_dev": [_P, _P, _U32, _U32, _P, _U32, _P, _U32, C.c_int32, _F, _P],
     "argmax_rows_f32_dev": [_P, _P, _U32, _U32, _P, _P, _U32, _U32, _P, _U32, _P],
     "u32_add_sat": [_P, _P, _U32, _U32, _U32, _U32],
+    "logits_adjust_rows_f32_dev": [_P, _P, _P, _U32, _U32, _P, _U32, _U32, _P, _U32] + [_P] * 5 + [_U32, _P, _P, _P],
+    "attention_decode_paged_dev": [_P] * 17 + [_U32] * 11 + [_F, _F],
+    "kv_pages_copy_f16": [_P] * 7 + [_U32] * 6 + [_I, _U32, C.POINTER(C.c_uint32)],
+    "kv_pages_evict": [_P] * 11 + [_U32] * 9,
     "reduce_ranks_add_f32": [_P, _P, _P, _P, _U32, _U32, _U32, _F],
     "exchange_add_ll_f32": [_P, _P, _P, _P, _U32],
     "prefetch_l2": [_P, _P, _U32],
@@ -222,6 +229,20 @@ def decode_attention_static_max_scratch() -> int:
     L = load_library()
     L.tm_cuda_attention_decode_static_max_scratch.restype = C.c_size_t
     return int(L.tm_cuda_attention_decode_static_max_scratch())
+
+
+def kv_pages_supported(head_dim: int, page_rows: int) -> bool:
+    L = load_library()
+    L.tm_cuda_kv_pages_supported.argtypes = [_U32] * 2
+    return bool(L.tm_cuda_kv_pages_supported(head_dim, page_rows))
+
+
+def attention_paged_scratch_bytes(n_seq: int, heads: int, kv_heads: int, head_dim: int, page_rows: int, max_pages: int,
+                                  weights: bool = False) -> int:
+    L = load_library()
+    L.tm_cuda_attention_paged_scratch_bytes.restype = C.c_size_t
+    L.tm_cuda_attention_paged_scratch_bytes.argtypes = [_U32] * 6 + [_I]
+    return int(L.tm_cuda_attention_paged_scratch_bytes(n_seq, heads, kv_heads, head_dim, page_rows, max_pages, int(weights)))
 
 
 def mma_workspace_bytes(cols: int, batch: int) -> int:
@@ -490,6 +511,38 @@ class CudaContext:
     def argmax_rows_dev(self, x, n_rows, n, partial, out, out_stride, base, pos_buf, out_cap, mirror=None):
         self._call("argmax_rows_f32_dev", x.handle, n_rows, n, partial.handle, out.handle, out_stride, base,
                    pos_buf.handle, out_cap, self._h(mirror))
+
+    def logits_adjust_rows(self, x, y, n_rows, n, log=None, log_stride=0, base=0, pos_buf=None, penalties=None,
+                           prompt_len=None, bias_ids=None, bias_values=None, bias_count=None, bias_cap=0, mask=None,
+                           partial=None, log_cap=None, mirror=None):
+        """Penalties, biases and a mask on rows of logits; with `partial` also the greedy choice, into the log."""
+        h = self._h
+        self._call("logits_adjust_rows_f32_dev", x.handle, y.handle, n_rows, n, h(log), log_stride, base, h(pos_buf),
+                   log_stride if log_cap is None else log_cap, h(prompt_len), h(penalties), h(bias_ids), h(bias_values),
+                   h(bias_count), bias_cap, h(mask), h(partial), h(mirror))
+
+    # a pool of cache pages shared by many sequences (include/tm_cuda.h)
+    def attention_decode_paged(self, q, k, v, q_norm, k_norm, inv_freq, k_pages, v_pages, table, out, scratch, pos_buf,
+                               len_buf, status, n_seq, heads, kv_heads, head_dim, n_rot, pages, page_rows, max_pages,
+                               window, eps, scale, q_stride=0, kv_stride=0, weights_in=None, weights_out=None):
+        self._call("attention_decode_paged_dev", q.handle, k.handle, v.handle, q_norm.handle, k_norm.handle,
+                   inv_freq.handle, k_pages.handle, v_pages.handle, table.handle, out.handle, scratch.handle,
+                   pos_buf.handle, len_buf.handle, status.handle, self._h(weights_in), self._h(weights_out), n_seq,
+                   q_stride, kv_stride, heads, kv_heads, head_dim, n_rot, pages, page_rows, max_pages, window, eps, scale)
+
+    def kv_pages_copy(self, k_cache, v_cache, k_pages, v_pages, table, status, pages, page_rows, max_pages, kv_heads,
+                      head_dim, cap, to_pages, runs):
+        """`runs`: (dense sequence, table row, first row, rows) of each run of rows."""
+        flat = [int(u) for r in runs for u in r]
+        self._call("kv_pages_copy_f16", k_cache.handle, v_cache.handle, k_pages.handle, v_pages.handle, table.handle,
+                   status.handle, pages, page_rows, max_pages, kv_heads, head_dim, cap, int(to_pages), len(runs),
+                   (C.c_uint32 * len(flat))(*flat))
+
+    def kv_pages_evict(self, k_pages, v_pages, table, to_table, len_buf, len_out, weights, weights_out, kept, status,
+                       n_seq, kv_heads, head_dim, pages, page_rows, max_pages, keep, first, recent):
+        self._call("kv_pages_evict", k_pages.handle, v_pages.handle, table.handle, to_table.handle, len_buf.handle,
+                   len_out.handle, weights.handle, weights_out.handle, kept.handle, status.handle, n_seq, kv_heads,
+                   head_dim, pages, page_rows, max_pages, keep, first, recent)
 
     def u32_add_sat(self, buf, first, count, delta, limit):
         self._call("u32_add_sat", buf.handle, first, count, delta, limit)
