@@ -646,10 +646,13 @@ int tm_cuda_argmax_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, uint32_t n_
  *   mask (may be NULL)       [n_rows][ceil(n / 32)] words; bit t % 32 of word t / 32 clear: -infinity.
  * With `partial` (n_rows * TM_CUDA_LOGITS_PARTIAL_BYTES) each row's largest logit that is neither masked nor NaN (ties to
  * the lowest index, 0xFFFFFFFF when there is none) goes to log[r * log_stride + base + pos_buf[r]], and to `mirror` when
- * given, if that slot is below log_cap <= log_stride.  n <= TM_CUDA_LOGITS_MAX.  Refused where an operand that is written
+ * given, if that slot is below log_cap <= log_stride.  n <= TM_CUDA_LOGITS_MAX; with penalties log_cap <=
+ * TM_CUDA_LOGITS_MAX_LOG; bias_cap <= TM_CUDA_LOGITS_MAX_BIASES.  Refused where an operand that is written
  * shares storage with another, but for y with x. */
 #define TM_CUDA_LOGITS_MAX (1u << 21)
-#define TM_CUDA_LOGITS_PARTIAL_BYTES 2048
+#define TM_CUDA_LOGITS_PARTIAL_BYTES 4096
+#define TM_CUDA_LOGITS_MAX_LOG ((1u << 20) - 1u)
+#define TM_CUDA_LOGITS_MAX_BIASES 4095u
 int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_cuda_buffer *y, uint32_t n_rows, uint32_t n,
                                        tm_cuda_buffer *log, uint32_t log_stride, uint32_t base, tm_cuda_buffer *pos_buf,
                                        uint32_t log_cap, tm_cuda_buffer *prompt_len, tm_cuda_buffer *penalties,

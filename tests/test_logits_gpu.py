@@ -202,7 +202,8 @@ def test_logits_refusals(ctx):
     for over in (dict(rows=0), dict(rows=65536), dict(n=0), dict(n=cuda.LOGITS_MAX + 1), dict(n=101), dict(rows=3), dict(log=None),
                  dict(pos_buf=None), dict(log_cap=0), dict(log_cap=11), dict(log_stride=11), dict(penalties=None),
                  dict(partial=None, mirror=log), dict(bias_values=None), dict(bias_ids=None), dict(bias_count=None),
-                 dict(bias_cap=0), dict(bias_cap=4), dict(mask=cnt), dict(partial=pen), dict(mirror=cnt), dict(mirror=log),
+                 dict(bias_cap=0), dict(bias_cap=4), dict(bias_cap=cuda.LOGITS_MAX_BIASES + 1),
+                 dict(log_cap=cuda.LOGITS_MAX_LOG + 1, log_stride=cuda.LOGITS_MAX_LOG + 1), dict(mask=cnt), dict(partial=pen), dict(mirror=cnt), dict(mirror=log),
                  dict(y=f.view(16, rows * n * 4 - 16)), dict(y=log), dict(partial=y), dict(x=part, n=4, y=part.view(16, 64))):
         with pytest.raises(cuda.CudaError) as e:
             call(**over)

@@ -2,17 +2,22 @@
 // grammar's mask, and the greedy choice among what is left.
 //
 // What bounds it: 8 bytes a logit (read once, written once) and an eighth for the mask.  A CTA takes a stretch of one row
-// whose per-token words (how often the log holds the token, which bias entry names it) fit in shared memory, so nothing
-// the size of the vocabulary is kept between calls or cleared: the CTA reads the row's whole log (a few kilobytes that the
-// row's CTAs share in L2) and counts the tokens of its own stretch with integer atomics, whose order does not matter.  Each
-// step of the arithmetic is rounded to f32 by itself, so a choice does not hang on how an expression was contracted.
+// whose per-token words fit in shared memory, so nothing the size of the vocabulary is kept between calls or cleared: the
+// CTA reads the row's whole log and bias map (a few kilobytes that the row's CTAs share in L2) and counts the tokens of its
+// own stretch with integer atomics, whose order does not matter, while its logits are on their way into registers.  The
+// arithmetic is done once for each named token, by the thread that holds it; all other logits pass from registers to memory
+// under the mask (words tested for every logit: 32 rows of 151936 34 us instead of 16.7; the log read once by a cluster of
+// CTAs that send each other its entries: 19.4).  Each step is rounded to f32 by itself, so a choice does not hang on how an
+// expression was contracted.
 #include "tm_cuda_internal.cuh"
 #include "tm_cuda_device.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr uint32_t kMostChunks = TM_CUDA_LOGITS_PARTIAL_BYTES / 8;
+constexpr uint32_t kCountBits = 20;
+static_assert(TM_CUDA_LOGITS_MAX_LOG < 1u << kCountBits && TM_CUDA_LOGITS_MAX_BIASES < 1u << (32 - kCountBits), "fit in a token's word");
+constexpr uint32_t kMostChunks = TM_CUDA_LOGITS_PARTIAL_BYTES / 8, kNone = 0xffffffffu;
 
 struct logits_args {
     const float *x;
@@ -20,13 +25,15 @@ struct logits_args {
     const uint32_t *log, *pos, *prompt, *bias_ids, *bias_count, *mask;
     const float *penalties, *bias_values;
     unsigned long long *partial;
-    uint32_t n, chunk, log_stride, base, bias_cap, mask_words, log_cap;
+    uint32_t n, log_stride, base, bias_cap, mask_words, log_cap;
+    bool quads;  // rows of x and y begin on 16 bytes
 };
 
-// (value, index) as one integer: larger values first, then lower indices; 0 is no entry.  -0 counts as +0.
-__device__ __forceinline__ unsigned long long choice_key(float v, uint32_t i) {
-    const uint32_t b = __float_as_uint(v + 0.0f), k = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (unsigned long long)k << 32 | (0xffffffffu - i);
+// Floats as integers in their order; -0 counts as +0, nothing but NaN maps to 0 .. 0x7fffff.  A (value, index) pair is one
+// integer, larger values first, then lower indices; 0 is no pair.
+__device__ __forceinline__ uint32_t order(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
 #pragma unroll
@@ -38,61 +45,157 @@ __device__ __forceinline__ uint32_t history(const logits_args &a, uint32_t r) {
     return (uint32_t)min((uint64_t)a.base + a.pos[r], (uint64_t)a.log_cap);
 }
 
-__global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const logits_args a) {
-    extern __shared__ uint32_t words[];  // [chunk] twice the count of generated tokens, + 1 where the prompt holds it
-    uint32_t *entry = words + a.chunk;   // [chunk] last bias entry that names the token, from 1
-    __shared__ unsigned long long best_of[kThreads / 32];
+// The best of a warp's (value, index) pairs, as the first lane's key.
+__device__ __forceinline__ unsigned long long warp_best(float v, uint32_t at) {
+    const uint32_t k = at == kNone ? 0u : order(v), top = __reduce_max_sync(0xffffffffu, k);
+    const uint32_t low = __reduce_min_sync(0xffffffffu, k == top ? at : kNone);
+    return top == 0u ? 0ull : (unsigned long long)top << 32 | (0xffffffffu - low);
+}
+
+// EACH quads of logits a thread: a stretch of EACH * 1024 logits.
+template <int EACH>
+__global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_kernel(const logits_args a) {
+    constexpr uint32_t kChunk = EACH * 4u * kThreads, kBatch = 8;
+    // Of each token: how often the log holds it from the prompt's end on, and above those bits its last bias entry, from 1.
+    __shared__ __align__(16) uint32_t words[kChunk];
+    __shared__ uint32_t logged[kChunk / 32], biased[kChunk / 32];  // a bit a token: the log holds it; the bias map names it
+    __shared__ unsigned long long keys[kThreads / 32];
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
-    const uint32_t r = blockIdx.y, c0 = blockIdx.x * a.chunk, m = min(a.chunk, a.n - c0), tid = threadIdx.x;
-    for (uint32_t i = tid; i < (a.bias_ids ? 2 : 1) * a.chunk; i += kThreads) words[i] = 0u;
-    __syncthreads();
-    float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
-    if (a.penalties) {
-        rep = a.penalties[r * 3];
-        presence = a.penalties[r * 3 + 1];
-        frequency = a.penalties[r * 3 + 2];
-        const uint32_t n = history(a, r), prompt = a.prompt ? a.prompt[r] : 0u;
-        const uint32_t *log = a.log + (size_t)r * a.log_stride;
-#pragma unroll 4
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const uint32_t at = log[i] - c0;
-            if (at < m) {
-                if (i < prompt) atomicOr(&words[at], 1u);
-                else atomicAdd(&words[at], 2u);
-            }
-        }
-    }
-    if (a.bias_ids) {
-        const uint32_t n = min(a.bias_count[r], a.bias_cap);
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const uint32_t at = a.bias_ids[(size_t)r * a.bias_cap + i] - c0;
-            if (at < m) atomicMax(&entry[at], i + 1u);
-        }
-    }
-    __syncthreads();
+    const uint32_t r = blockIdx.y, c0 = blockIdx.x * kChunk, m = min(kChunk, a.n - c0), tid = threadIdx.x;
     const float *x = a.x + (size_t)r * a.n + c0;
     float *y = a.y + (size_t)r * a.n + c0;
-    unsigned long long best = 0ull;
-    for (uint32_t i = tid; i < m; i += kThreads) {
-        float v = x[i];
-        const uint32_t word = words[i], count = word >> 1, e = a.bias_ids ? entry[i] : 0u;
-        if (word != 0u) v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-        if (count != 0u) v = __fsub_rn(__fsub_rn(v, __fmul_rn(frequency, (float)count)), presence);
-        if (e != 0u) v = __fadd_rn(v, a.bias_values[(size_t)r * a.bias_cap + e - 1u]);
-        const uint32_t t = c0 + i;
-        const bool allowed = !a.mask || (a.mask[(size_t)r * a.mask_words + t / 32u] >> (t & 31u) & 1u);
-        if (!allowed) v = -INFINITY;
-        y[i] = v;
-        if (allowed && !isnan(v)) best = max(best, choice_key(v, t));
+    const uint32_t *mask = a.mask ? a.mask + (size_t)r * a.mask_words + c0 / 32u : nullptr;
+    const uint32_t *log = a.log + (size_t)r * a.log_stride, *ids = a.bias_ids + (size_t)r * a.bias_cap;
+    // The first entries of the log and of the bias map are asked for before the row's lengths have arrived.
+    uint32_t log_id[kBatch], bias_id = a.bias_ids && tid < a.bias_cap ? ids[tid] : kNone;
+#pragma unroll
+    for (uint32_t u = 0; u < kBatch; ++u) log_id[u] = a.penalties && u * kThreads + tid < a.log_cap ? log[u * kThreads + tid] : kNone;
+    const uint32_t n_log = a.penalties ? history(a, r) : 0u, prompt = a.penalties && a.prompt ? a.prompt[r] : 0u;
+    const uint32_t n_bias = a.bias_ids ? min(a.bias_count[r], a.bias_cap) : 0u;
+    float v[EACH][4];
+    uint32_t allowed = 0u;  // a bit a logit of this thread: the mask lets it through
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const uint32_t i = (e * kThreads + tid) * 4u;
+        if (a.quads) {
+            if (i < m) *(float4 *)v[e] = *(const float4 *)(x + i);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[e][k] = i + k < m ? x[i + k] : 0.0f;
+        }
     }
-    if (!a.partial) return;
-    best = warp_max(best);
-    if ((tid & 31u) == 0u) best_of[tid >> 5] = best;
+    const bool any = a.penalties || a.bias_ids;
+    if (any) {
+        for (uint32_t i = tid * 4u; i < kChunk; i += kThreads * 4u) *(uint4 *)(words + i) = make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t i = tid; i < kChunk / 32; i += kThreads) logged[i] = biased[i] = 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const uint32_t i = (e * kThreads + tid) * 4u;
+        if (i < m) allowed |= ((mask ? mask[i / 32u] >> (i & 31u) : 15u) & 15u) << (4 * e);
+    }
+    if (any) {
+        __syncthreads();
+        if (a.bias_ids) {
+            for (uint32_t i = tid; i < n_bias; i += kThreads) {
+                const uint32_t at = (i == tid ? bias_id : ids[i]) - c0;
+                if (at >= m) continue;
+                atomicOr(&biased[at / 32u], 1u << (at & 31u));
+                atomicMax(&words[at], (i + 1u) << kCountBits);
+            }
+            __syncthreads();
+        }
+        for (uint32_t i0 = tid; i0 < n_log; i0 += kBatch * kThreads) {  // kBatch loads on their way at a time
+            if (i0 != tid) {
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) log_id[u] = i0 + u * kThreads < n_log ? log[i0 + u * kThreads] : kNone;
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                const uint32_t at = log_id[u] - c0, i = i0 + u * kThreads;
+                if (at < m && i < n_log) {
+                    atomicOr(&logged[at / 32u], 1u << (at & 31u));
+                    if (i >= prompt) atomicAdd(&words[at], 1u);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // ---- the logits that nothing names; the others are stored as they are ----
+    float best = -INFINITY;
+    // The best's quad; a bit a logit of this thread: a candidate here, named.
+    uint32_t best_quad = 0u, mine = 0u, others = 0u;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const uint32_t i = (e * kThreads + tid) * 4u;
+        if (i >= m) continue;
+        const uint32_t in = m - i < 4u ? (1u << (m - i)) - 1u : 15u, named = any ? (logged[i / 32u] | biased[i / 32u]) >> (i & 31u) & in : 0u;
+        const uint32_t let = allowed >> (4 * e), can = let & ~named & in, show = let | named;
+        mine |= can << (4 * e);
+        others |= named << (4 * e);
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            top = fmaxf(top, can >> k & 1u ? v[e][k] : -INFINITY);  // (a NaN is passed over)
+            v[e][k] = show >> k & 1u ? v[e][k] : -INFINITY;
+        }
+        if (top > best) {
+            best = top;
+            best_quad = e;
+        }
+        if (a.quads) {
+            *(float4 *)(y + i) = *(const float4 *)v[e];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < m) y[i + k] = v[e][k];
+        }
+    }
+    uint32_t best_at = kNone;
+    if (a.partial && mine != 0u) {
+        const bool found = best > -INFINITY;  // else the first that is -infinity and no NaN, whatever its quad
+#pragma unroll
+        for (int e = EACH - 1; e >= 0; --e)
+#pragma unroll
+            for (int k = 3; k >= 0; --k)
+                if (v[e][k] == best && (mine >> (4 * e + k) & 1u) != 0u && (!found || best_quad == e)) best_at = c0 + (e * kThreads + tid) * 4u + k;
+    }
+    // ---- the others, by the thread that holds them ----
+    const float repetition = a.penalties ? a.penalties[r * 3] : 1.0f, presence = a.penalties ? a.penalties[r * 3 + 1] : 0.0f;
+    const float frequency = a.penalties ? a.penalties[r * 3 + 2] : 0.0f;
+#pragma unroll 1
+    for (; others != 0u; others &= others - 1u) {
+        const uint32_t j = __ffs(others) - 1u, at = ((j >> 2) * kThreads + tid) * 4u + (j & 3u);
+        float tree[EACH * 4];
+#pragma unroll
+        for (int i = 0; i < EACH * 4; ++i) tree[i] = v[i / 4][i % 4];
+#pragma unroll
+        for (int half = EACH * 2; half > 0; half >>= 1)
+#pragma unroll
+            for (int i = 0; i < half; ++i) tree[i] = j & half ? tree[i + half] : tree[i];
+        float z = tree[0];
+        const uint32_t word = words[at], count = word & ((1u << kCountBits) - 1u), entry = word >> kCountBits;
+        const float bias = entry != 0u ? a.bias_values[(size_t)r * a.bias_cap + entry - 1u] : 0.0f;
+        if (logged[at / 32u] >> (at & 31u) & 1u) {
+            z = z > 0.0f ? __fdiv_rn(z, repetition) : __fmul_rn(z, repetition);
+            if (count != 0u) z = __fsub_rn(__fsub_rn(z, __fmul_rn(frequency, (float)count)), presence);
+        }
+        if (entry != 0u) z = __fadd_rn(z, bias);
+        const bool can = (allowed >> j & 1u) != 0u;
+        y[at] = can ? z : -INFINITY;
+        if (can && !isnan(z) && (best_at == kNone || z > best || (z == best && c0 + at < best_at))) {
+            best = z;
+            best_at = c0 + at;
+        }
+    }
+    if (!a.partial || m == 0u) return;
+    const unsigned long long key = warp_best(best, best_at);
+    if ((tid & 31u) == 0u) keys[tid >> 5] = key;
     __syncthreads();
     if (tid < 32u) {
-        best = warp_max(tid < kThreads / 32 ? best_of[tid] : 0ull);
-        if (tid == 0u) a.partial[(size_t)r * kMostChunks + blockIdx.x] = best;
+        const unsigned long long top = warp_max(tid < kThreads / 32 ? keys[tid] : 0ull);
+        if (tid == 0u) a.partial[(size_t)r * kMostChunks + blockIdx.x] = top;
     }
 }
 
@@ -108,10 +211,15 @@ __global__ void __launch_bounds__(32) logits_choose_kernel(const unsigned long l
     best = warp_max(best);
     const uint64_t slot = (uint64_t)base + pos[r];
     if (threadIdx.x == 0 && slot < log_cap) {
-        const uint32_t id = best ? 0xffffffffu - (uint32_t)best : 0xffffffffu;
+        const uint32_t id = best ? 0xffffffffu - (uint32_t)best : kNone;
         log[(size_t)r * log_stride + slot] = id;
         if (mirror) mirror[(size_t)r * log_stride + slot] = id;
     }
+}
+
+template <int EACH>
+cudaError_t launch_adjust(tm_cuda_ctx *ctx, const logits_args &a, uint32_t chunks, uint32_t n_rows) {
+    return tm_launch_pdl(ctx, logits_adjust_kernel<EACH>, dim3(chunks, n_rows), dim3(kThreads), 0, a);
 }
 
 }  // namespace
@@ -133,11 +241,15 @@ int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_c
         return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "penalties and a choice need the token logs and positions");
     if (uses_log && (log_cap == 0 || log_cap > log_stride))
         return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "token log of %u slots in rows of %u", log_cap, log_stride);
+    if (penalties && log_cap > TM_CUDA_LOGITS_MAX_LOG)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "penalties over token logs of %u slots (at most %u)", log_cap, (unsigned)TM_CUDA_LOGITS_MAX_LOG);
     if (prompt_len && !penalties)
         return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "prompt lengths are for penalties");
     if (mirror && !partial) return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "a mirror is for a choice");
     if ((bias_ids || bias_values || bias_count) && (!bias_ids || !bias_values || !bias_count || bias_cap == 0))
         return tm_fail(err, err_cap, TM_CUDA_ERR_UNSUPPORTED, "a bias map is ids, values and counts of at most %u entries", bias_cap);
+    if (bias_ids && bias_cap > TM_CUDA_LOGITS_MAX_BIASES)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "bias maps of %u entries (at most %u)", bias_cap, (unsigned)TM_CUDA_LOGITS_MAX_BIASES);
     const uint32_t words = (n + 31u) / 32u;
     const size_t nx = (size_t)n_rows * n * 4, nlog = ((size_t)(n_rows - 1) * log_stride + log_cap) * 4, nr = (size_t)n_rows * 4;
     const size_t nbias = (size_t)n_rows * bias_cap * 4, nmask = (size_t)n_rows * words * 4;
@@ -181,18 +293,25 @@ int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_c
     a.bias_values = bias_values ? (const float *)bias_values->dev : nullptr;
     a.partial = partial ? (unsigned long long *)partial->dev : nullptr;
     a.n = n;
-    a.chunk = n <= 1024u * kMostChunks ? 1024u : (n + kMostChunks - 1) / kMostChunks;
+    a.quads = n % 4u == 0u && (((size_t)x->dev | (size_t)y->dev) & 15u) == 0u;
     a.log_stride = log_stride;
     a.base = base;
     a.bias_cap = bias_cap;
     a.mask_words = words;
     a.log_cap = log_cap;
-    const uint32_t chunks = (n + a.chunk - 1) / a.chunk;
-    const size_t smem = (size_t)a.chunk * 4 * (bias_ids ? 2 : 1);
-    if (smem > 48u * 1024u)  // (more than 1.5 million logits with a bias map: at most 64 KB)
-        TM_CUDA_TRY(cudaFuncSetAttribute(logits_adjust_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // Stretches of 1024 logits keep every SM busy with one row (151936 logits, a log of 600: 4.2 us); with many rows longer
+    // ones, because every CTA reads the row's log (32 rows of 151936, logs up to 4000, a mask and a bias map: 2048 logits
+    // 20.9 us, 4096 16.8, 8192 16.7; 48 of 262144, logs up to 1200: 36.6, 29.6, 27.4, floor 15.7).
+    const uint32_t most = 4u * (uint32_t)ctx->sm_count;
+    uint32_t each = 1;
+    while (each < 8u && ((n + each * 1024u - 1) / (each * 1024u) > kMostChunks || (uint64_t)n_rows * ((n + each * 1024u - 1) / (each * 1024u)) > most))
+        each *= 2;
+    const uint32_t chunks = (n + each * 1024u - 1) / (each * 1024u);
     TM_OP_BEGIN("logits_adjust_rows");
-    TM_CUDA_TRY(tm_launch_pdl(ctx, logits_adjust_kernel, dim3(chunks, n_rows), dim3(kThreads), smem, a));
+    TM_CUDA_TRY(each == 1   ? launch_adjust<1>(ctx, a, chunks, n_rows)
+                : each == 2 ? launch_adjust<2>(ctx, a, chunks, n_rows)
+                : each == 4 ? launch_adjust<4>(ctx, a, chunks, n_rows)
+                            : launch_adjust<8>(ctx, a, chunks, n_rows));
     if (partial)
         TM_CUDA_TRY(tm_launch_pdl(ctx, logits_choose_kernel, dim3(n_rows), dim3(32), 0, (const unsigned long long *)a.partial,
                                   chunks, (uint32_t *)log->dev, log_stride, base, a.pos, log_cap,

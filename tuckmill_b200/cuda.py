@@ -26,7 +26,8 @@ EPI_STORE, EPI_ADD, EPI_SILU_MUL_F16, EPI_GELU_MUL_F16 = 0, 1, 2, 3
 STATUS_PAST_CAPACITY, STATUS_LATE, STATUS_BAD_PAGE = 1, 2, 4
 SEQ_NONE = 0xFFFFFFFF
 PAGED_MAX_SEQUENCES = 1024
-LOGITS_MAX, LOGITS_PARTIAL_BYTES = 1 << 21, 2048
+LOGITS_MAX, LOGITS_PARTIAL_BYTES = 1 << 21, 4096
+LOGITS_MAX_LOG, LOGITS_MAX_BIASES = (1 << 20) - 1, 4095
 
 
 class CudaError(RuntimeError):
