@@ -12,12 +12,14 @@ def test_shapes_that_pages_serve():
             assert cuda.kv_pages_supported(hd, page) == (hd in (32, 64, 128, 256) and page in (16, 32, 64, 128, 256))
 
 
-def test_scratch_grows_with_counted_rows_only():
+def test_scratch_of_a_call():
     plain = cuda.attention_paged_scratch_bytes(4, 16, 8, 128, 64, 100)
-    assert plain == cuda.attention_paged_scratch_bytes(900, 64, 8, 128, 16, 7) > 0  # what CTAs leave behind
+    assert plain == cuda.attention_paged_scratch_bytes(4, 16, 8, 128, 16, 7) > 0  # without weights the cache's length is no matter
     counted = cuda.attention_paged_scratch_bytes(4, 16, 8, 128, 64, 100, True)
-    assert counted == plain + 4 * 16 * 4 * (2 + 6400)  # a score a row and head, a maximum and a sum a head
+    assert counted == plain + 4 * 16 * 4 * 6400  # a score a row and head
     assert cuda.attention_paged_scratch_bytes(1024, 1024, 32, 256, 256, 1 << 17, True) > 1 << 47  # no 32-bit product
+    for heads, kvh, hd, page in ((3, 2, 64, 16), (4, 0, 64, 16), (4, 2, 48, 16), (4, 2, 64, 24)):
+        assert cuda.attention_paged_scratch_bytes(1, heads, kvh, hd, page, 4) == 0
 
 
 @pytest.mark.parametrize("name,args", [

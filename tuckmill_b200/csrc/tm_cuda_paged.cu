@@ -57,11 +57,13 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // What bounds it: the cached rows' bytes, 4 head_dim per row and KV head.  So every row is read once for all (up to
 // eight) query heads of its group, and the machine's bandwidth is shared out evenly however ragged the lengths are:
 // the tiles of 64 rows of all (sequence, KV head) pairs form one line, and CTA i of G takes the i-th of G equal runs of
-// it.  A pair that falls into one run is finished there; pieces of the others meet in a second, small launch.
+// it.  Three launches: the vectors (queries and new rows: norm, rotation, f16), the rows, and the join of what the warps
+// have found.  The second starts beside the first and waits for it when it has its rows on their way.
 //
-// A warp takes 16 rows of each tile through its own ring of cp.async stages and keeps its own running (max, sum, output),
-// so the warps of a CTA do not meet before the end of a run.  Both products are mma.m16n8k16 with the cached rows as the
-// 16-row operand and the heads as the 8 columns: S^T = K Q^T, then O^T = V^T P^T, with P transposed in registers.
+// A warp takes 16 rows of each tile through its own ring of cp.async stages and keeps its own running (max, sum, output):
+// the warps of a CTA never meet (with the pieces of a pair combined in the CTA, barriers and the next pair's queries took
+// 7000 cycles a pair, as long as 250 rows).  The ring runs on across pairs.  Both products are mma.m16n8k16 with the cached
+// rows as the 16-row operand and the heads as the 8 columns: S^T = K Q^T, then O^T = V^T P^T, with P transposed in registers.
 //
 // Accuracy: cached rows are f16, so their products with f16 operands are exact in f32.  Q and P are split into a sum of two
 // f16 each (22 bits; Q against a power of two at its largest element, P in units of 2^-14, so that neither runs out of
@@ -69,7 +71,6 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // results are those of 32-bit arithmetic.  The second multiply hides behind the loads.
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr uint32_t kBlock = 16, kTile = kBlock * kAttnWarps;
-constexpr uint32_t kMostCtas = 640;
 constexpr float kUnit = 14.0f;  // P and its sums are held times 2^14
 
 template <int HD>
@@ -78,16 +79,25 @@ struct attn_cfg {
     static constexpr uint32_t kPlane = kBlock * PITCH, kStage = 2 * kPlane;  // a warp's 16 keys, then its 16 values
     static constexpr int kStages = HD > 64 ? 3 : 4;
     static constexpr int kCtas = HD == 256 ? 1 : HD == 128 ? 2 : 3;  // an SM
-    static constexpr int QP = HD + 8;                                // halves a row of Q: distinct banks for 8 rows
     static constexpr uint32_t kRing = kAttnWarps * kStages * kStage;
-    static constexpr uint32_t kBytes = kRing + 2 * 8 * QP * 2 + 2 * HD * 2 + 9 * HD * 4 + (8 + 2 * kAttnWarps * 8) * 4;
+    static constexpr uint32_t kQ = HD / 16 * 32 * 16;  // a pair's queries as operands: 16 bytes a lane and 16 dims
+    static constexpr bool kQRegs = HD <= 128;          // held in registers, else a copy a warp in shared memory
+    static constexpr uint32_t kBytes = kRing + (kQRegs ? 0u : kAttnWarps * kQ);
 };
+// CTAs of a launch, for which the scratch has room: one to three on each of up to 160 SMs.
+constexpr uint32_t most_ctas(uint32_t head_dim) { return 160u * (head_dim == 256 ? 1u : head_dim == 128 ? 2u : 3u); }
 
 struct paged_args {
     const float *q, *k, *v, *q_norm, *k_norm, *inv_freq;
     __half *kp, *vp;
     const uint32_t *table, *pos, *len;
-    float *out, *part, *scores, *ml;  // scores, ml: only where weights are counted
+    float *out, *scores;  // scores: only where weights are counted
+    uint4 *ops;           // [sequence][pair][16 dims][lane]: the pair's queries as the multiply's operand, high and low halves
+    float *factor;        // [sequence][pair][8]: what makes a product of those a score in units of log 2
+    // The warps' outputs and (max, sum): of a pair that goes on from another CTA or into one [CTA][0: goes on, 1: begins][8][warp],
+    // of a pair that one CTA has whole [sequence][head][warp].
+    float *part, *whole;
+    float2 *part_ml, *whole_ml;
     const float *w_in;
     float *w_out;
     uint32_t *status;
@@ -119,221 +129,247 @@ __device__ __forceinline__ uint32_t sharers(uint64_t T, const paged_args &a) { r
 // Which CTA owns tile t of T: the i with i T / G <= t < (i + 1) T / G, whole numbers throughout.
 __device__ __forceinline__ uint32_t cta_of(uint64_t t, uint64_t T, uint32_t G) { return (uint32_t)(((t + 1) * G - 1) / T); }
 
+// A tile of the line.
+struct cursor {
+    uint32_t s, pair, t, nt, len, start;
+    __device__ __forceinline__ void enter(const paged_args &a) {
+        len = a.len[s];
+        nt = pair_tiles(len, a);
+        start = first_row(len, a.window);
+    }
+    // To the next pair; behind the last one of all it stays at a sequence that is none.
+    __device__ __forceinline__ void next_pair(const paged_args &a) {
+        t = 0;
+        if (++pair < a.kv_heads * a.blocks) return;
+        pair = 0;
+        for (++s; s < a.n_seq; ++s) {
+            enter(a);
+            if (nt != 0u) break;
+        }
+    }
+};
+
+// The vectors: a warp norms and rotates one query head, or a KV head's new key, and stores it.  Its latency is hidden by
+// nothing, so everything it needs is asked for at once.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const paged_args a) {
+    constexpr int EPL = HD / 32;
+    __shared__ float rows[8][HD];
+    tmdev::pdl_wait();
+    tmdev::pdl_trigger();  // the next kernel may read what those before this one have written
+    const uint32_t warp = tmdev::warp_index(), lane = threadIdx.x & 31u, per = a.heads + a.kv_heads;
+    const uint64_t at = (uint64_t)blockIdx.x * 8u + warp;
+    const uint32_t s = (uint32_t)(at / per), x = (uint32_t)(at % per);
+    if (s >= a.n_seq) return;
+    const bool is_k = x >= a.heads;
+    const uint32_t kvh = x - a.heads, len = a.len[s], pos = a.pos[s];
+    const float *src = is_k ? a.k + (size_t)s * a.kv_stride + (size_t)kvh * HD : a.q + (size_t)s * a.q_stride + (size_t)x * HD;
+    const float *nw = is_k ? a.k_norm : a.q_norm, *vs = a.v + (size_t)s * a.kv_stride + (size_t)kvh * HD;
+    float y[EPL], w[EPL], v[EPL], ss = 0.0f;
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) {
+        y[r] = src[lane + 32 * r];
+        w[r] = nw[lane + 32 * r];
+        v[r] = is_k ? vs[lane + 32 * r] : 0.0f;
+    }
+    if (len >= a.cap) {
+        if (x == 0u && lane == 0 && len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) ss = fmaf(y[r], y[r], ss);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+    float *row = rows[warp];
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = y[r] * inv * w[r];
+    __syncwarp();
+    const uint32_t half = a.n_rot / 2u;
+    for (uint32_t i = lane; i < half; i += 32u) {
+        const float angle = (float)pos * a.inv_freq[i], c = cosf(angle), sn = sinf(angle);
+        const float x0 = row[i], x1 = row[i + half];
+        row[i] = x0 * c - x1 * sn;
+        row[i + half] = x0 * sn + x1 * c;
+    }
+    __syncwarp();
+    if (is_k) {
+        const uint32_t id = a.table[(size_t)s * a.max_pages + (len >> a.page_log)];
+        if (id >= a.pages) {
+            if (lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+            return;
+        }
+        const size_t to = ((((size_t)id * a.kv_heads + kvh) << a.page_log) + (len & ((1u << a.page_log) - 1u))) * HD;
+#pragma unroll
+        for (int r = 0; r < EPL; ++r) {
+            a.kp[to + lane + 32 * r] = __float2half_rn(row[lane + 32 * r]);
+            a.vp[to + lane + 32 * r] = __float2half_rn(v[r]);
+        }
+        return;
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) top = fmaxf(top, fabsf(row[lane + 32 * r]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // q = 2^e (hi + lo), |hi| < 2; a vector of zeros, infinities or NaN keeps e = 0
+    int e = (int)((__float_as_uint(top) >> 23) & 0xffu) - 127;
+    e = top > 0.0f && top < INFINITY ? max(-120, min(120, e)) : 0;
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const uint32_t in_group = x % a.group, h = in_group % 8u;
+    const size_t pair = (size_t)s * a.kv_heads * a.blocks + x / a.group * a.blocks + in_group / 8u;
+    if (lane == 0) a.factor[pair * 8 + h] = a.scale_log2e * __uint_as_float((uint32_t)(127 + e) << 23);
+    for (uint32_t i = lane; i < HD / 4; i += 32u) {  // lane 4 h + t of the operand for 16 dims: dims 2t, 2t + 1, 2t + 8, 2t + 9
+        const float *d = row + i / 4u * 16u + i % 4u * 2u;
+        const float z0 = d[0] * down, z1 = d[1] * down, z2 = d[8] * down, z3 = d[9] * down;
+        const __half2 h0 = __floats2half2_rn(z0, z1), h1 = __floats2half2_rn(z2, z3);
+        const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+        a.ops[(pair * (HD / 16) + i / 4u) * 32 + h * 4u + i % 4u] =
+            make_uint4(bits(h0), bits(h1), bits(__floats2half2_rn(z0 - f0.x, z1 - f0.y)), bits(__floats2half2_rn(z2 - f1.x, z3 - f1.y)));
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_paged_kernel(const paged_args a) {
     using C = attn_cfg<HD>;
-    constexpr int PITCH = C::PITCH, STAGES = C::kStages, QP = C::QP, EPL = HD / 32;
+    constexpr int PITCH = C::PITCH, STAGES = C::kStages, KT = HD / 16;
     extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char *ring = smem;
-    __half *q_hi = (__half *)(smem + C::kRing), *q_lo = q_hi + 8 * QP;
-    __half *k_new = q_lo + 8 * QP, *v_new = k_new + HD;
-    float *vec = (float *)(v_new + HD);  // a head vector per warp and iteration, for the rotation's pairs
-    float *factor = vec + 9 * HD, *wm = factor + 8, *wl = wm + kAttnWarps * 8;
-    const uint32_t tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t warp = tmdev::warp_index(), lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t ring = smem_addr(smem) + warp * (STAGES * C::kStage);
+    uint4 *const q_copy = (uint4 *)(smem + C::kRing + (C::kQRegs ? 0u : warp * C::kQ));
     tmdev::pdl_trigger();
-    tmdev::pdl_wait();
 
+    // ---- this CTA's run of tiles ----
     const uint32_t pairs = a.kv_heads * a.blocks;
     const uint64_t T = tiles_before(a.n_seq, a);
-    if (blockIdx.x == 0 && warp == 0)
-        for (uint32_t s = lane; s < a.n_seq; s += 32u)
-            if (a.len[s] >= a.cap && a.len[s] != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
     const uint32_t G = sharers(T, a);
-    if (blockIdx.x >= G) return;
-    uint64_t u = blockIdx.x * T / G;
-    const uint64_t u1 = (blockIdx.x + 1ull) * T / G;
-    // The sequence that tile u belongs to, and the tiles before it.
-    uint32_t s = 0;
-    uint64_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32u) {
-        uint64_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) : 0u, incl = n;
+    if (blockIdx.x >= G) {
+        tmdev::pdl_wait();
+        return;
+    }
+    const uint64_t u0 = blockIdx.x * T / G;
+    uint32_t left = (uint32_t)((blockIdx.x + 1ull) * T / G - u0);
+    cursor at;
+    {
+        uint64_t before = 0;  // tiles of the sequences before the one that tile u0 belongs to
+        at.s = 0;
+        for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32u) {
+            const uint64_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) : 0u;
+            uint64_t incl = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= (uint32_t)o) incl += up;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= (uint32_t)o) incl += up;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + incl * pairs > u0);
+            if (past) {
+                const int first = __ffs(past) - 1;
+                at.s = s0 + first;
+                before += __shfl_sync(0xffffffffu, incl - n, first) * pairs;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31) * pairs;
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, before + incl * pairs > u);
-        if (past) {
-            const int at = __ffs(past) - 1;
-            s = s0 + at;
-            before += __shfl_sync(0xffffffffu, incl - n, at) * pairs;
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31) * pairs;
+        at.enter(a);
+        at.pair = (uint32_t)((u0 - before) / at.nt);
+        at.t = (uint32_t)((u0 - before) % at.nt);
     }
 
-    const uint32_t ring_base = smem_addr(ring) + warp * (STAGES * C::kStage);
-    while (u < u1) {
-        const uint32_t len = tmdev::uniform(a.len[s]), nt = pair_tiles(len, a);
-        if (nt == 0u) {
-            ++s;
-            continue;
-        }
-        const uint32_t start = first_row(len, a.window);
-        const uint32_t pair = (uint32_t)((u - before) / nt), t0 = (uint32_t)((u - before) % nt);
-        const uint32_t tn = (uint32_t)min((uint64_t)(nt - t0), u1 - u);
-        const uint32_t kvh = pair / a.blocks, hb = pair % a.blocks;
-        const uint32_t head0 = kvh * a.group + hb * 8u, heads = min(8u, a.group - hb * 8u);
-        const uint32_t block0 = (start / kTile + t0) * kAttnWarps + warp;  // this warp's first 16 rows; then every 4th
-        const uint32_t *pages = a.table + (size_t)s * a.max_pages;
-        const bool owns_new = t0 + tn == nt;
-
-        // ---- the ring of cached rows ----
-        auto in_sight = [&](uint32_t blk) { return blk * kBlock <= len && blk * kBlock + (kBlock - 1u) >= start; };
-        auto page_of = [&](uint32_t i) {  // of this warp's i-th block
-            const uint32_t blk = block0 + i * kAttnWarps;
-            return i < tn && in_sight(blk) ? pages[blk * kBlock >> a.page_log] : 0u;
-        };
-        auto load = [&](uint32_t i, uint32_t id) {
-            const uint32_t blk = block0 + i * kAttnWarps;
-            if (i < tn && in_sight(blk)) {
-                const bool page = id < a.pages;
+    // ---- the ring of cached rows: `ahead` is the tile whose page was asked for last, `coming` tiles are not on their way ----
+    const uint32_t page_low = (1u << a.page_log) - 1u;
+    cursor ahead = at;
+    uint32_t coming = left, ahead_id = 0u, fill = 0u;
+    bool waited = false;
+    auto wait = [&] {  // for the vectors
+        if (!waited) tmdev::pdl_wait();
+        waited = true;
+    };
+    auto block_of = [&](const cursor &c) { return (c.start / kTile + c.t) * kAttnWarps + warp; };
+    auto in_sight = [](const cursor &c, uint32_t blk) { return blk * kBlock <= c.len && blk * kBlock + (kBlock - 1u) >= c.start; };
+    auto ask = [&] {
+        const uint32_t blk = block_of(ahead);
+        ahead_id = in_sight(ahead, blk) ? a.table[(size_t)ahead.s * a.max_pages + (blk * kBlock >> a.page_log)] : 0u;
+    };
+    auto load = [&](bool first) {
+        if (coming != 0u) {
+            const uint32_t blk = block_of(ahead);
+            if (in_sight(ahead, blk)) {
+                if (first && ahead.len - blk * kBlock < kBlock) wait();  // the new row is among these
+                const bool page = ahead_id < a.pages;
                 if (!page && lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
-                const size_t row0 = (((size_t)(page ? id : 0u) * a.kv_heads + kvh) << a.page_log) +
-                                    (blk * kBlock & ((1u << a.page_log) - 1u));
-                const uint32_t dst = ring_base + (i % STAGES) * C::kStage;
+                const uint32_t kvh = ahead.pair / a.blocks;
+                const size_t row0 = (((size_t)(page ? ahead_id : 0u) * a.kv_heads + kvh) << a.page_log) + (blk * kBlock & page_low);
+                const uint32_t dst = ring + fill * C::kStage;
 #pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
+                for (int c = 0; c < KT; ++c) {
                     const uint32_t e = c * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), j = blk * kBlock + r;
-                    const bool live = page && j >= start && j < len;  // the rest is zeros; row `len` comes from this call
+                    const bool live = page && j >= ahead.start && j <= ahead.len;  // the rest is zeros
                     cp_async16(dst + sw<PITCH>(r, ch), a.kp + (row0 + r) * HD + ch * 8u, live);
                     cp_async16(dst + C::kPlane + sw<PITCH>(r, ch), a.vp + (row0 + r) * HD + ch * 8u, live);
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) load(i, page_of(i));
-        uint32_t next_id = page_of(STAGES - 1);
+            if (--coming != 0u) {
+                if (++ahead.t >= ahead.nt) ahead.next_pair(a);
+                ask();
+            }
+        }
+        fill = fill + 1u == STAGES ? 0u : fill + 1u;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    ask();
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) load(true);
+    wait();
 
-        // ---- the group's queries, and the new row where this run ends with it: norm, rotation, f16 ----
-        const uint32_t pos = a.pos[s];
-        for (uint32_t x = warp; x < heads + (owns_new ? 1u : 0u); x += kAttnWarps) {
-            const bool is_k = x == heads;
-            const float *src = is_k ? a.k + (size_t)s * a.kv_stride + (size_t)kvh * HD
-                                    : a.q + (size_t)s * a.q_stride + (size_t)(head0 + x) * HD;
-            const float *nw = is_k ? a.k_norm : a.q_norm;
-            float y[EPL], ss = 0.0f;
+    uint32_t stage = 0u;
+#pragma unroll 1
+    while (left != 0u) {
+        // ---- a run of one pair's tiles ----
+        const uint32_t s = at.s, len = at.len, start = at.start, tn = min(at.nt - at.t, left);
+        const uint32_t kvh = at.pair / a.blocks, hb = at.pair % a.blocks;
+        const uint32_t head0 = kvh * a.group + hb * 8u, heads = min(8u, a.group - hb * 8u);
+        const bool begins = at.t == 0u, ends = at.t + tn == at.nt;
+        const size_t pair = (size_t)s * pairs + at.pair;
+        // (columns of no head hold what the scratch holds: a column of the products depends on nothing but its own)
+        uint4 qr[C::kQRegs ? KT : 1];
 #pragma unroll
-            for (int r = 0; r < EPL; ++r) {
-                y[r] = src[lane + 32 * r];
-                ss = fmaf(y[r], y[r], ss);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
-            float *row = vec + x * HD;
-#pragma unroll
-            for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = y[r] * inv * nw[lane + 32 * r];
-            __syncwarp();
-            const uint32_t half = a.n_rot / 2u;
-            for (uint32_t i = lane; i < half; i += 32u) {
-                const float angle = (float)pos * a.inv_freq[i], c = cosf(angle), sn = sinf(angle);
-                const float x0 = row[i], x1 = row[i + half];
-                row[i] = x0 * c - x1 * sn;
-                row[i + half] = x0 * sn + x1 * c;
-            }
-            __syncwarp();
-            float top = 0.0f;
-#pragma unroll
-            for (int r = 0; r < EPL; ++r) {
-                y[r] = row[lane + 32 * r];
-                top = fmaxf(top, fabsf(y[r]));
-            }
-            if (is_k) {
-                const uint32_t id = pages[len >> a.page_log];
-                const bool page = id < a.pages;
-                if (!page && lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
-                const size_t at = ((((size_t)(page ? id : 0u) * a.kv_heads + kvh) << a.page_log) + (len & ((1u << a.page_log) - 1u))) * HD;
-                const float *vs = a.v + (size_t)s * a.kv_stride + (size_t)kvh * HD;
-#pragma unroll
-                for (int r = 0; r < EPL; ++r) {
-                    const uint32_t e = lane + 32 * r;
-                    const __half hk = __float2half_rn(y[r]), hv = __float2half_rn(vs[e]);
-                    k_new[e] = hk;
-                    v_new[e] = hv;
-                    if (page && hb == 0u) {
-                        a.kp[at + e] = hk;
-                        a.vp[at + e] = hv;
-                    }
-                }
-                continue;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // q = 2^e (hi + lo), |hi| < 2; a vector of zeros, infinities or NaN keeps e = 0
-            int e = (int)((__float_as_uint(top) >> 23) & 0xffu) - 127;
-            e = top > 0.0f && top < INFINITY ? max(-120, min(120, e)) : 0;
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-            for (int r = 0; r < EPL; ++r) {
-                const float z = y[r] * down;
-                const __half hi = __float2half_rn(z);
-                q_hi[x * QP + lane + 32 * r] = hi;
-                q_lo[x * QP + lane + 32 * r] = __float2half_rn(z - __half2float(hi));
-            }
-            if (lane == 0) factor[x] = a.scale_log2e * __uint_as_float((uint32_t)(127 + e) << 23);
+        for (int kt = 0; kt < KT; ++kt) {
+            const uint4 v = a.ops[(pair * KT + kt) * 32 + lane];
+            if (C::kQRegs) qr[C::kQRegs ? kt : 0] = v;
+            else q_copy[kt * 32 + lane] = v;  // (each lane reads back its own)
         }
-        for (uint32_t x = heads + warp; x < 8u; x += kAttnWarps) {  // columns of no head
-            for (uint32_t e = lane; e < HD; e += 32u) q_hi[x * QP + e] = q_lo[x * QP + e] = __float2half_rn(0.0f);
-            if (lane == 0) factor[x] = 0.0f;
-        }
-        __syncthreads();
-        uint32_t qh[HD <= 128 ? HD / 16 : 1][2], ql[HD <= 128 ? HD / 16 : 1][2];
-        if (HD <= 128) {
+        const float f0 = a.factor[pair * 8 + 2 * t], f1 = a.factor[pair * 8 + 2 * t + 1];
+        float o[KT][4];
 #pragma unroll
-            for (int kt = 0; kt < (HD <= 128 ? HD / 16 : 1); ++kt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    qh[kt][i] = *(const uint32_t *)(q_hi + g * QP + kt * 16 + i * 8 + 2 * t);
-                    ql[kt][i] = *(const uint32_t *)(q_lo + g * QP + kt * 16 + i * 8 + 2 * t);
-                }
-        }
-        const float f0 = factor[2 * t], f1 = factor[2 * t + 1];
-        float o[HD / 16][4];
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < KT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;  // heads 2t and 2t + 1; l: this lane's rows
+        float *scores = a.scores ? a.scores + ((size_t)s * a.kv_heads + kvh) * a.cap * a.group + hb * 8u + 2 * t : nullptr;
 
 #pragma unroll 1
         for (uint32_t i = 0; i < tn; ++i) {
-            const uint32_t blk = block0 + i * kAttnWarps, j0 = blk * kBlock;
+            const uint32_t j0 = ((start / kTile + at.t + i) * kAttnWarps + warp) * kBlock;
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();  // this block has landed for all lanes, and all have read the one before it
-            load(i + STAGES - 1, next_id);
-            next_id = page_of(i + STAGES);
-            if (!in_sight(blk)) continue;
-            const uint32_t kb = ring_base + (i % STAGES) * C::kStage, vb = kb + C::kPlane;
-            if (len - j0 < kBlock) {  // the new row
-                unsigned char *st = ring + (kb - smem_addr(ring));
-                if (lane < HD / 8) {
-                    *(uint4 *)(st + sw<PITCH>(len - j0, lane)) = *(const uint4 *)(k_new + lane * 8);
-                    *(uint4 *)(st + C::kPlane + sw<PITCH>(len - j0, lane)) = *(const uint4 *)(v_new + lane * 8);
-                }
-                __syncwarp();
-            }
+            load(false);
+            const uint32_t kb = ring + stage * C::kStage, vb = kb + C::kPlane;
+            stage = stage + 1u == STAGES ? 0u : stage + 1u;
+            if (j0 > len || j0 + (kBlock - 1u) < start) continue;
             float hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int kt = 0; kt < HD / 16; ++kt) {
+            for (int kt = 0; kt < KT; ++kt) {
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4(kb + sw<PITCH>(lane & 15u, kt * 2 + (lane >> 4)), a0, a1, a2, a3);
-                if (HD <= 128) {
-                    mma_f16(hi, a0, a1, a2, a3, qh[kt % (HD <= 128 ? HD / 16 : 1)][0], qh[kt % (HD <= 128 ? HD / 16 : 1)][1]);
-                    mma_f16(lo, a0, a1, a2, a3, ql[kt % (HD <= 128 ? HD / 16 : 1)][0], ql[kt % (HD <= 128 ? HD / 16 : 1)][1]);
-                } else {
-                    const __half *qp = q_hi + g * QP + kt * 16 + 2 * t;
-                    mma_f16(hi, a0, a1, a2, a3, *(const uint32_t *)qp, *(const uint32_t *)(qp + 8));
-                    qp += 8 * QP;
-                    mma_f16(lo, a0, a1, a2, a3, *(const uint32_t *)qp, *(const uint32_t *)(qp + 8));
-                }
+                const uint4 b = C::kQRegs ? qr[C::kQRegs ? kt : 0] : q_copy[kt * 32 + lane];
+                mma_f16(hi, a0, a1, a2, a3, b.x, b.y);
+                mma_f16(lo, a0, a1, a2, a3, b.z, b.w);
             }
             // rows j0 + g and j0 + g + 8, heads 2t and 2t + 1
             const uint32_t ja = j0 + g, jb = ja + 8u;
             const bool see_a = ja >= start && ja <= len, see_b = jb >= start && jb <= len;
             const float s0 = see_a ? (hi[0] + lo[0]) * f0 : -INFINITY, s1 = see_a ? (hi[1] + lo[1]) * f1 : -INFINITY;
             const float s2 = see_b ? (hi[2] + lo[2]) * f0 : -INFINITY, s3 = see_b ? (hi[3] + lo[3]) * f1 : -INFINITY;
-            if (a.scores) {
-                float *row = a.scores + (((size_t)s * a.kv_heads + kvh) * a.cap + ja) * a.group + hb * 8u + 2 * t;
+            if (scores) {
+                float *row = scores + (size_t)ja * a.group;
                 if (see_a && 2 * t < heads) row[0] = s0;
                 if (see_a && 2 * t + 1 < heads) row[1] = s1;
                 row += (size_t)8 * a.group;
@@ -348,12 +384,12 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             }
             x0 = fmaxf(x0, m0);
             x1 = fmaxf(x1, m1);
-            const float u0 = (x0 == -INFINITY ? 0.0f : x0), u1m = (x1 == -INFINITY ? 0.0f : x1);
-            const float al0 = exp2f(m0 - u0), al1 = exp2f(m1 - u1m);
+            const float d0 = x0 == -INFINITY ? 0.0f : x0, d1 = x1 == -INFINITY ? 0.0f : x1;
+            const float al0 = exp2f(m0 - d0), al1 = exp2f(m1 - d1);
             m0 = x0;
             m1 = x1;
-            const float p0 = exp2f(s0 - u0 + kUnit), p1 = exp2f(s1 - u1m + kUnit);
-            const float p2 = exp2f(s2 - u0 + kUnit), p3 = exp2f(s3 - u1m + kUnit);
+            const float p0 = exp2f(s0 - d0 + kUnit), p1 = exp2f(s1 - d1 + kUnit);
+            const float p2 = exp2f(s2 - d0 + kUnit), p3 = exp2f(s3 - d1 + kUnit);
             l0 = fmaf(l0, al0, p0 + p2);
             l1 = fmaf(l1, al1, p1 + p3);
             const __half2 pa = __floats2half2_rn(p0, p1), pb = __floats2half2_rn(p2, p3);
@@ -363,7 +399,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             const uint32_t r1 = transpose8x8(bits(__floats2half2_rn(p2 - fb.x, p3 - fb.y)));
             const uint32_t mat = lane >> 3, vr = (lane & 7u) + (mat >> 1) * 8u;
 #pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt) {
+            for (int mt = 0; mt < KT; ++mt) {
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4_t(vb + sw<PITCH>(vr, mt * 2 + (mat & 1u)), a0, a1, a2, a3);
                 float d[4] = {0, 0, 0, 0};
@@ -375,135 +411,143 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
                 o[mt][3] = fmaf(o[mt][3], al1, d[3]);
             }
         }
-        // ---- the warps' states -> this run's ----
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();  // the ring is free
-        float *wo = (float *)ring;  // [warps][8][HD]
+        // ---- what this warp has found (zeros, where it saw no row) ----
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
             l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
         }
-        if (g == 0) {
-            wm[warp * 8 + 2 * t] = m0;
-            wm[warp * 8 + 2 * t + 1] = m1;
-            wl[warp * 8 + 2 * t] = l0;
-            wl[warp * 8 + 2 * t + 1] = l1;
-        }
+        const bool whole = begins && ends;
+        const size_t piece = whole ? ((size_t)s * a.heads + head0) * kAttnWarps + warp
+                                   : ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * 8 * kAttnWarps + warp;  // of head 0; then every 4th
+        float *to = whole ? a.whole : a.part;
+        float2 *ml = whole ? a.whole_ml : a.part_ml;
 #pragma unroll
-        for (int mt = 0; mt < HD / 16; ++mt)
+        for (uint32_t e = 0; e < 2u; ++e) {
+            const uint32_t h = 2 * t + e;
+            if (h >= heads) continue;
+            if (g == 0) ml[piece + h * kAttnWarps] = e ? make_float2(m1, l1) : make_float2(m0, l0);
+            float *row = to + (piece + h * kAttnWarps) * HD + g;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                wo[(warp * 8 + 2 * t + (e & 1)) * HD + mt * 16 + g + (e >> 1) * 8] = o[mt][e];
-        __syncthreads();
-        const bool whole = tn == nt;
-        float *part = a.part + ((size_t)blockIdx.x * 2 + (t0 == 0u ? 1 : 0)) * 8 * (HD + 2);
-        for (uint32_t i = tid; i < heads * HD; i += kAttnThreads) {
-            const uint32_t h = i / HD, d = i % HD;
-            float M = wm[h];
-#pragma unroll
-            for (int w = 1; w < kAttnWarps; ++w) M = fmaxf(M, wm[w * 8 + h]);
-            const float top = M == -INFINITY ? 0.0f : M;
-            float L = 0.0f, O = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
-                const float f = exp2f(wm[w * 8 + h] - top);  // a warp that saw no row: 0
-                L = fmaf(f, wl[w * 8 + h], L);
-                O = fmaf(f, wo[(w * 8 + h) * HD + d], O);
-            }
-            if (whole) a.out[((size_t)s * a.heads + head0 + h) * HD + d] = O / L;
-            else part[h * (HD + 2) + 2 + d] = O;
-            if (d == 0) {
-                float *ml = whole ? (a.ml ? a.ml + ((size_t)s * a.heads + head0 + h) * 2 : nullptr) : part + h * (HD + 2);
-                if (ml) {
-                    ml[0] = M;
-                    ml[1] = L;
-                }
+            for (int mt = 0; mt < KT; ++mt) {
+                row[mt * 16] = o[mt][e];
+                row[mt * 16 + 8] = o[mt][2 + e];
             }
         }
-        __syncthreads();
-        u += tn;
-        if (u - before == (uint64_t)nt * pairs) {
-            before = u;
-            ++s;
-        }
+        left -= tn;
+        if (left != 0u) at.next_pair(a);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Joins the pieces of pairs that more than one CTA had a run of (grid.z 0), and counts the attention of 1024 rows a CTA
-// (grid.z from 1 on).
-constexpr uint32_t kJoinThreads = 256, kCountRows = 1024;
+// Joins the warps' pieces of every pair (a CTA a head, a warp a piece), and counts the attention of 1024 rows a CTA (the
+// CTAs behind those).
+constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kCountRows = 1024;
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(const paged_args a) {
-    __shared__ float sm[32], sl[32];
+    constexpr int EPL = HD / 32;
+    __shared__ float sm[32], sl[32], so[kJoinWarps][HD];
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
-    const uint32_t s = blockIdx.y, tid = threadIdx.x, len = a.len[s], nt = pair_tiles(len, a);
+    const uint32_t s = blockIdx.y, tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u;
+    const uint32_t len = a.len[s], nt = pair_tiles(len, a);
     if (nt == 0u) return;
     const uint64_t T = tiles_before(a.n_seq, a), before = tiles_before(s, a);
     const uint32_t G = sharers(T, a);
-    const size_t stride = 8 * (HD + 2);
-    // Partial result c of a pair whose first tile is u: CTA i0 has begun it, the others carry on.
-    auto piece = [&](uint32_t i0, uint32_t i) { return a.part + ((size_t)i * 2 + (i == i0 ? 1 : 0)) * stride; };
-    if (blockIdx.z == 0) {
-        const uint32_t pair = blockIdx.x, kvh = pair / a.blocks, hb = pair % a.blocks;
-        const uint32_t head0 = kvh * a.group + hb * 8u, heads = min(8u, a.group - hb * 8u);
-        const uint64_t u = before + (uint64_t)pair * nt;
-        const uint32_t i0 = cta_of(u, T, G), i1 = cta_of(u + nt - 1, T, G);
-        if (i0 == i1) return;
-        for (uint32_t e = tid; e < heads * HD; e += kJoinThreads) {
-            const uint32_t h = e / HD, d = e % HD;
-            float M = -INFINITY, L = 0.0f, O = 0.0f;
-            for (uint32_t c0 = i0; c0 <= i1; c0 += 8) {
-                float mb[8], lb[8], ob[8];
+    // The pieces of a head: `n` of them, 4 a CTA; CTA i0 has begun the pair, the others carry on.
+    struct pieces {
+        uint32_t i0, n, h;
+        bool whole;
+        size_t base;
+        __device__ __forceinline__ size_t operator[](uint32_t i) const {
+            return whole ? base + i : ((size_t)(i0 + i / kAttnWarps) * 2 + (i < (uint32_t)kAttnWarps ? 1 : 0)) * 8 * kAttnWarps + h * kAttnWarps + i % kAttnWarps;
+        }
+    };
+    auto of = [&](uint32_t head) {
+        const uint32_t kvh = head / a.group, in_group = head % a.group;
+        const uint64_t u = before + (uint64_t)(kvh * a.blocks + in_group / 8u) * nt;
+        pieces p;
+        p.i0 = cta_of(u, T, G);
+        p.n = (cta_of(u + nt - 1, T, G) - p.i0 + 1u) * kAttnWarps;
+        p.whole = p.n == (uint32_t)kAttnWarps;
+        p.h = in_group % 8u;
+        p.base = ((size_t)s * a.heads + head) * kAttnWarps;
+        return p;
+    };
+    if (blockIdx.x < a.heads) {
+        const uint32_t head = blockIdx.x;
+        const pieces p = of(head);
+        const float *rows = p.whole ? a.whole : a.part;
+        const float2 *mls = p.whole ? a.whole_ml : a.part_ml;
+        float M = -INFINITY, L = 0.0f, O[EPL];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float *p = piece(i0, min(c0 + c, i1)) + h * (HD + 2);
-                    mb[c] = c0 + c <= i1 ? p[0] : -INFINITY;
-                    lb[c] = p[1];
-                    ob[c] = p[2 + d];
-                }
-                float top = M;
+        for (int r = 0; r < EPL; ++r) O[r] = 0.0f;
+        for (uint32_t i = warp; i < p.n; i += 4 * kJoinWarps) {
+            float2 ml[4];
+            float ob[4][EPL];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) top = fmaxf(top, mb[c]);
-                const float use = top == -INFINITY ? 0.0f : top, al = exp2f(M - use);
-                L *= al;
-                O *= al;
+            for (int c = 0; c < 4; ++c) {
+                const size_t x = p[min(i + c * kJoinWarps, p.n - 1u)];
+                ml[c] = mls[x];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    if (c0 + c > i1) break;
-                    const float f = exp2f(mb[c] - use);
-                    L = fmaf(f, lb[c], L);
-                    O = fmaf(f, ob[c], O);
-                }
-                M = top;
+                for (int r = 0; r < EPL; ++r) ob[c][r] = rows[x * HD + lane + 32 * r];
             }
-            a.out[((size_t)s * a.heads + head0 + h) * HD + d] = O / L;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (i + c * kJoinWarps >= p.n) break;
+                const float top = fmaxf(M, ml[c].x), use = top == -INFINITY ? 0.0f : top;
+                const float al = exp2f(M - use), f = exp2f(ml[c].x - use);  // a warp that saw no row: 0
+                M = top;
+                L = fmaf(L, al, f * ml[c].y);
+#pragma unroll
+                for (int r = 0; r < EPL; ++r) O[r] = fmaf(O[r], al, f * ob[c][r]);
+            }
+        }
+        if (lane == 0) {
+            sm[warp] = M;
+            sl[warp] = L;
+        }
+#pragma unroll
+        for (int r = 0; r < EPL; ++r) so[warp][lane + 32 * r] = O[r];
+        __syncthreads();
+        if (tid < HD) {
+            float top = sm[0];
+#pragma unroll
+            for (uint32_t w = 1; w < kJoinWarps; ++w) top = fmaxf(top, sm[w]);
+            const float use = top == -INFINITY ? 0.0f : top;
+            float l = 0.0f, o = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kJoinWarps; ++w) {
+                const float f = exp2f(sm[w] - use);  // a warp that had no piece: 0
+                l = fmaf(f, sl[w], l);
+                o = fmaf(f, so[w][tid], o);
+            }
+            a.out[((size_t)s * a.heads + head) * HD + tid] = o / l;
         }
         return;
     }
-    const uint32_t row0 = (blockIdx.z - 1u) * kCountRows;
-    if (blockIdx.x % a.blocks != 0u || row0 > len) return;
-    const uint32_t kvh = blockIdx.x / a.blocks;
-    if (tid < a.group) {
-        const uint32_t hb = tid / 8u, h = tid % 8u;
-        const uint64_t u = before + (uint64_t)(kvh * a.blocks + hb) * nt;
-        const uint32_t i0 = cta_of(u, T, G), i1 = cta_of(u + nt - 1, T, G);
+    const uint32_t kvh = (blockIdx.x - a.heads) % a.kv_heads, row0 = (blockIdx.x - a.heads) / a.kv_heads * kCountRows;
+    if (row0 > len) return;
+    for (uint32_t x = warp; x < a.group; x += kJoinWarps) {  // a head's maximum and sum, a lane a piece
+        const pieces p = of(kvh * a.group + x);
+        const float2 *mls = p.whole ? a.whole_ml : a.part_ml;
         float M = -INFINITY, L = 0.0f;
-        if (i0 == i1) {
-            const float *ml = a.ml + ((size_t)s * a.heads + kvh * a.group + tid) * 2;
-            M = ml[0];
-            L = ml[1];
-        } else {
-            for (uint32_t i = i0; i <= i1; ++i) M = fmaxf(M, piece(i0, i)[h * (HD + 2)]);
-            const float use = M == -INFINITY ? 0.0f : M;
-            for (uint32_t i = i0; i <= i1; ++i) {
-                const float *p = piece(i0, i) + h * (HD + 2);
-                L = fmaf(exp2f(p[0] - use), p[1], L);
-            }
+        for (uint32_t i = lane; i < p.n; i += 32u) {
+            const float2 ml = mls[p[i]];
+            const float top = fmaxf(M, ml.x), use = top == -INFINITY ? 0.0f : top;
+            L = fmaf(L, exp2f(M - use), exp2f(ml.x - use) * ml.y);
+            M = top;
         }
-        sm[tid] = M - kUnit;
-        sl[tid] = L;
+        float top = M;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        L *= exp2f(M - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane == 0) {
+            sm[x] = top - kUnit;
+            sl[x] = L;
+        }
     }
     __syncthreads();
     const uint32_t start = first_row(len, a.window);
@@ -519,8 +563,25 @@ __global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(cons
     }
 }
 
+// Where the parts of the scratch lie, in bytes; `end` is its size.
+struct scratch_parts {
+    size_t ops, factor, part, part_ml, whole, whole_ml, scores, end;
+    scratch_parts(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint64_t cap, bool weights) {
+        const size_t pairs = (size_t)n_seq * kv_heads * ((heads / kv_heads + 7u) / 8u), rows = (size_t)n_seq * heads * kAttnWarps;
+        const size_t pieces = (size_t)most_ctas(head_dim) * 2 * 8 * kAttnWarps;
+        ops = 0;
+        factor = ops + pairs * (head_dim / 16) * 32 * 16;
+        part = factor + pairs * 32;
+        part_ml = part + pieces * head_dim * 4;
+        whole = part_ml + pieces * 8;
+        whole_ml = whole + rows * head_dim * 4;
+        scores = whole_ml + rows * 8;
+        end = scores + (weights ? (size_t)n_seq * heads * cap * 4 : 0);
+    }
+};
+
 template <int HD>
-cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a, uint64_t &kernels) {
+cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
     using C = attn_cfg<HD>;
     static std::atomic<bool> attr_done[64] = {};  // per device; contexts of a process share it
     const int device = ctx->device;
@@ -529,16 +590,15 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a, uint64_t &kernels) {
         if (e != cudaSuccess) return e;
         if (device >= 0 && device < 64) attr_done[device].store(true, std::memory_order_release);
     }
-    const uint64_t tiles = ((uint64_t)a.cap + kTile - 1) / kTile, pairs = (uint64_t)a.n_seq * a.kv_heads * a.blocks;
-    const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), kMostCtas);
-    a.ctas = (uint32_t)(pairs * tiles < places ? pairs * tiles : places);
-    cudaError_t e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
-    kernels = 1;
-    if (e == cudaSuccess && (tiles > 1 || a.w_out)) {  // (pairs of one tile are never cut)
-        const uint32_t z = a.w_out ? 1u + (a.cap + kCountRows - 1) / kCountRows : 1u;
-        e = tm_launch_pdl(ctx, attention_paged_join_kernel<HD>, dim3(a.kv_heads * a.blocks, a.n_seq, z), dim3(kJoinThreads), 0, a);
-        kernels = 2;
-    }
+    const uint64_t tiles = ((uint64_t)a.cap + kTile - 1) / kTile * a.n_seq * a.kv_heads * a.blocks;
+    const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), most_ctas(HD));
+    a.ctas = (uint32_t)(tiles < places ? tiles : places);
+    const uint64_t vectors = (uint64_t)a.n_seq * (a.heads + a.kv_heads);
+    cudaError_t e = tm_launch_pdl(ctx, attention_paged_vectors_kernel<HD>, dim3((uint32_t)((vectors + 7) / 8)), dim3(256), 0, a);
+    if (e == cudaSuccess) e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
+    const uint32_t count = a.w_out ? a.kv_heads * ((a.cap + kCountRows - 1) / kCountRows) : 0u;
+    if (e == cudaSuccess)
+        e = tm_launch_pdl(ctx, attention_paged_join_kernel<HD>, dim3(a.heads + count, a.n_seq), dim3(kJoinThreads), 0, a);
     return e;
 }
 
@@ -811,12 +871,10 @@ extern "C" {
 
 int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows) { return pages_ok(head_dim, page_rows) ? 1 : 0; }
 
-// Partial results of CTAs' runs; then, where attention is counted, (max, sum) of every head and the scores of every row.
 size_t tm_cuda_attention_paged_scratch_bytes(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                              uint32_t page_rows, uint32_t max_pages, int weights) {
-    (void)kv_heads;
-    const size_t part = (size_t)kMostCtas * 2 * 8 * (head_dim + 2) * 4;
-    return weights ? part + (size_t)n_seq * heads * 4 * (2 + (size_t)max_pages * page_rows) : part;
+    if (kv_heads == 0 || heads % kv_heads != 0 || !pages_ok(head_dim, page_rows)) return 0;
+    return scratch_parts(n_seq, heads, kv_heads, head_dim, (uint64_t)max_pages * page_rows, weights != 0).end;
 }
 
 int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_cuda_buffer *k, tm_cuda_buffer *v,
@@ -884,10 +942,15 @@ int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_c
     a.pos = (const uint32_t *)pos_buf->dev;
     a.len = (const uint32_t *)len_buf->dev;
     a.out = (float *)out->dev;
-    a.part = (float *)scratch->dev;
+    const scratch_parts at(n_seq, heads, kv_heads, head_dim, cap, weights_out != nullptr);
+    a.ops = (uint4 *)(scratch->dev + at.ops);
+    a.factor = (float *)(scratch->dev + at.factor);
+    a.part = (float *)(scratch->dev + at.part);
+    a.part_ml = (float2 *)(scratch->dev + at.part_ml);
+    a.whole = (float *)(scratch->dev + at.whole);
+    a.whole_ml = (float2 *)(scratch->dev + at.whole_ml);
     if (weights_out) {
-        a.ml = a.part + (size_t)kMostCtas * 2 * 8 * (head_dim + 2);
-        a.scores = a.ml + (size_t)n_seq * heads * 2;
+        a.scores = (float *)(scratch->dev + at.scores);
         a.w_in = weights_in ? (const float *)weights_in->dev : nullptr;
         a.w_out = (float *)weights_out->dev;
     }
@@ -908,12 +971,11 @@ int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_c
     a.eps = eps;
     a.scale_log2e = scale * 1.4426950408889634f;
     TM_OP_BEGIN("attention_decode_paged");
-    uint64_t kernels = 0;
-    TM_CUDA_TRY(head_dim == 32    ? launch_paged<32>(ctx, a, kernels)
-                : head_dim == 64  ? launch_paged<64>(ctx, a, kernels)
-                : head_dim == 128 ? launch_paged<128>(ctx, a, kernels)
-                                  : launch_paged<256>(ctx, a, kernels));
-    TM_OP_END(kernels);
+    TM_CUDA_TRY(head_dim == 32    ? launch_paged<32>(ctx, a)
+                : head_dim == 64  ? launch_paged<64>(ctx, a)
+                : head_dim == 128 ? launch_paged<128>(ctx, a)
+                                  : launch_paged<256>(ctx, a));
+    TM_OP_END(3);
 }
 
 int tm_cuda_kv_pages_copy_f16(tm_cuda_ctx *ctx, tm_cuda_buffer *k_cache, tm_cuda_buffer *v_cache, tm_cuda_buffer *k_pages,
