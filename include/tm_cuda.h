@@ -681,7 +681,8 @@ int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows);
  * f16).  The new key, normed and rotated at position pos_buf[s], and the new value are stored at row len_buf[s], and the
  * token attends rows start .. len_buf[s], start = len + 1 > window ? len + 1 - window : 0 (window 0: all).  The two buffers
  * may be one; they differ once rows have been evicted, and a window then counts rows.  Rows of q start q_stride elements
- * apart, of k and v kv_stride (0 = dense); out is [n_seq][heads * head_dim]; heads / kv_heads <= 32.
+ * apart, of k and v kv_stride (0 = dense); out is [n_seq][heads * head_dim]; heads / kv_heads <= 32; the sequences' tiles of
+ * 64 rows, of every KV head and eight of its query heads, are fewer than 2^32.
  * weights_out (may be NULL): [n_seq][kv_heads][max_pages * page_rows] f32, the attention that each row has drawn:
  * weights_in (NULL: zeros; may be weights_out) plus the sum of the softmax weights that the KV head's query heads give it
  * now.  The new row starts from 0; entries behind it are left as they are.

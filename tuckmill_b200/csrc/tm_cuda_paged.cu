@@ -113,21 +113,27 @@ __device__ __forceinline__ uint32_t first_row(uint32_t len, uint32_t window) {
 __device__ __forceinline__ uint32_t pair_tiles(uint32_t len, const paged_args &a) {
     return len >= a.cap ? 0u : len / kTile - first_row(len, a.window) / kTile + 1u;
 }
-__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-// Tiles of all sequences' pairs before sequence `upto` (whole warps call it).
-__device__ __forceinline__ uint64_t tiles_before(uint32_t upto, const paged_args &a) {
-    uint64_t n = 0;
+// The line of all pairs' tiles and the CTAs that share it, each with one tile at least, so that the pieces of a pair lie in
+// consecutive CTAs: CTA i has `each` tiles, or one more if i < extra.  (Entry point: T < 2^32.)
+struct line {
+    uint32_t ctas, each, extra;
+    __device__ __forceinline__ line(uint32_t T, const paged_args &a) {
+        ctas = min(T, a.ctas);
+        each = ctas != 0u ? T / ctas : 0u;
+        extra = T - each * ctas;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t i) const { return i * each + min(i, extra); }
+    __device__ __forceinline__ uint32_t owner(uint32_t t) const {
+        const uint32_t longer = extra * (each + 1u);
+        return t < longer ? t / (each + 1u) : extra + (t - longer) / each;
+    }
+};
+// Tiles of one head's pairs of the sequences below `upto` (whole warps call it).
+__device__ __forceinline__ uint32_t tiles_before(uint32_t upto, const paged_args &a) {
+    uint32_t n = 0;
     for (uint32_t s = threadIdx.x & 31u; s < upto; s += 32u) n += pair_tiles(a.len[s], a);
-    return warp_sum(n) * (a.kv_heads * a.blocks);
+    return __reduce_add_sync(0xffffffffu, n);
 }
-// The CTAs that share T tiles: each has one at least, so the pieces of a pair lie in consecutive CTAs.
-__device__ __forceinline__ uint32_t sharers(uint64_t T, const paged_args &a) { return (uint32_t)min(T, (uint64_t)a.ctas); }
-// Which CTA owns tile t of T: the i with i T / G <= t < (i + 1) T / G, whole numbers throughout.
-__device__ __forceinline__ uint32_t cta_of(uint64_t t, uint64_t T, uint32_t G) { return (uint32_t)(((t + 1) * G - 1) / T); }
 
 // A tile of the line.
 struct cursor {
@@ -241,38 +247,37 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
 
     // ---- this CTA's run of tiles ----
     const uint32_t pairs = a.kv_heads * a.blocks;
-    const uint64_t T = tiles_before(a.n_seq, a);
-    const uint32_t G = sharers(T, a);
-    if (blockIdx.x >= G) {
+    const line all(tiles_before(a.n_seq, a) * pairs, a);
+    if (blockIdx.x >= all.ctas) {
         tmdev::pdl_wait();
         return;
     }
-    const uint64_t u0 = blockIdx.x * T / G;
-    uint32_t left = (uint32_t)((blockIdx.x + 1ull) * T / G - u0);
+    const uint32_t u0 = all.begin(blockIdx.x);
+    uint32_t left = all.begin(blockIdx.x + 1u) - u0;
     cursor at;
     {
-        uint64_t before = 0;  // tiles of the sequences before the one that tile u0 belongs to
+        uint32_t before = 0;  // tiles of the sequences before the one that tile u0 belongs to
         at.s = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32u) {
-            const uint64_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) : 0u;
-            uint64_t incl = n;
+            const uint32_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) * pairs : 0u;
+            uint32_t incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= (uint32_t)o) incl += up;
             }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + incl * pairs > u0);
+            const uint32_t past = __ballot_sync(0xffffffffu, before + incl > u0);
             if (past) {
                 const int first = __ffs(past) - 1;
                 at.s = s0 + first;
-                before += __shfl_sync(0xffffffffu, incl - n, first) * pairs;
+                before += __shfl_sync(0xffffffffu, incl - n, first);
                 break;
             }
-            before += __shfl_sync(0xffffffffu, incl, 31) * pairs;
+            before += __shfl_sync(0xffffffffu, incl, 31);
         }
         at.enter(a);
-        at.pair = (uint32_t)((u0 - before) / at.nt);
-        at.t = (uint32_t)((u0 - before) % at.nt);
+        at.pair = (u0 - before) / at.nt;
+        at.t = (u0 - before) % at.nt;
     }
 
     // ---- the ring of cached rows: `ahead` is the tile whose page was asked for last, `coming` tiles are not on their way ----
@@ -440,60 +445,76 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Joins the warps' pieces of every pair (a CTA a head, a warp a piece), and counts the attention of 1024 rows a CTA (the
+// Joins the warps' pieces of every pair (a CTA a head, a warp a piece), and counts the attention of stretches of rows (the
 // CTAs behind those).
-constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kCountRows = 1024;
-template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(const paged_args a) {
-    constexpr int EPL = HD / 32;
+constexpr uint32_t kCountEach = 4;
+template <int HD, uint32_t kJoinWarps>
+__global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(const paged_args a) {
+    constexpr int EPL = HD / 32, kBatch = 4;
+    constexpr uint32_t kJoinThreads = 32 * kJoinWarps, kCountRows = kCountEach * kJoinThreads;
     __shared__ float sm[32], sl[32], so[kJoinWarps][HD];
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
     const uint32_t s = blockIdx.y, tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u;
     const uint32_t len = a.len[s], nt = pair_tiles(len, a);
     if (nt == 0u) return;
-    const uint64_t T = tiles_before(a.n_seq, a), before = tiles_before(s, a);
-    const uint32_t G = sharers(T, a);
+    const bool joins = blockIdx.x < a.heads;
+    const uint32_t kvh = joins ? blockIdx.x / a.group : (blockIdx.x - a.heads) % a.kv_heads;
+    const uint32_t row0 = joins ? 0u : (blockIdx.x - a.heads) / a.kv_heads * kCountRows, start = first_row(len, a.window);
+    if (row0 > len) return;
+    // What the rows have drawn before and the first four heads' scores are asked for before the pieces are known.
+    const size_t base = ((size_t)s * a.kv_heads + kvh) * a.cap;
+    float w[kCountEach], z[kCountEach][4];
+    if (!joins) {
+#pragma unroll
+        for (uint32_t r = 0; r < kCountEach; ++r) {
+            const uint32_t j = row0 + r * kJoinThreads + tid;
+            w[r] = a.w_in && j < len ? a.w_in[base + j] : 0.0f;  // the new row has drawn nothing before
+#pragma unroll
+            for (uint32_t h = 0; h < 4u; ++h) z[r][h] = h < a.group && j >= start && j <= len ? a.scores[(base + j) * a.group + h] : 0.0f;
+        }
+    }
+    const uint32_t pairs = a.kv_heads * a.blocks;
+    const line all(tiles_before(a.n_seq, a) * pairs, a);
+    const uint32_t before = tiles_before(s, a) * pairs;
     // The pieces of a head: `n` of them, 4 a CTA; CTA i0 has begun the pair, the others carry on.
     struct pieces {
-        uint32_t i0, n, h;
+        uint32_t n;
         bool whole;
         size_t base;
-        __device__ __forceinline__ size_t operator[](uint32_t i) const {
-            return whole ? base + i : ((size_t)(i0 + i / kAttnWarps) * 2 + (i < (uint32_t)kAttnWarps ? 1 : 0)) * 8 * kAttnWarps + h * kAttnWarps + i % kAttnWarps;
+        __device__ __forceinline__ size_t operator[](uint32_t i) const {  // (the first CTA's lie a block of 8 heads further on)
+            const uint32_t cta = i / kAttnWarps;
+            return base + (whole || cta == 0u ? 0u : (cta * 2u - 1u) * 8u * kAttnWarps) + i % kAttnWarps;
         }
     };
     auto of = [&](uint32_t head) {
-        const uint32_t kvh = head / a.group, in_group = head % a.group;
-        const uint64_t u = before + (uint64_t)(kvh * a.blocks + in_group / 8u) * nt;
+        const uint32_t in_group = head % a.group, u = before + (kvh * a.blocks + in_group / 8u) * nt, i0 = all.owner(u);
         pieces p;
-        p.i0 = cta_of(u, T, G);
-        p.n = (cta_of(u + nt - 1, T, G) - p.i0 + 1u) * kAttnWarps;
+        p.n = (all.owner(u + nt - 1u) - i0 + 1u) * kAttnWarps;
         p.whole = p.n == (uint32_t)kAttnWarps;
-        p.h = in_group % 8u;
-        p.base = ((size_t)s * a.heads + head) * kAttnWarps;
+        p.base = p.whole ? ((size_t)s * a.heads + head) * kAttnWarps : ((size_t)i0 * 2 + 1) * 8 * kAttnWarps + in_group % 8u * kAttnWarps;
         return p;
     };
-    if (blockIdx.x < a.heads) {
-        const uint32_t head = blockIdx.x;
-        const pieces p = of(head);
+    if (joins) {
+        const pieces p = of(blockIdx.x);
         const float *rows = p.whole ? a.whole : a.part;
         const float2 *mls = p.whole ? a.whole_ml : a.part_ml;
         float M = -INFINITY, L = 0.0f, O[EPL];
 #pragma unroll
         for (int r = 0; r < EPL; ++r) O[r] = 0.0f;
-        for (uint32_t i = warp; i < p.n; i += 4 * kJoinWarps) {
-            float2 ml[4];
-            float ob[4][EPL];
+        for (uint32_t i = warp; i < p.n; i += kBatch * kJoinWarps) {
+            float2 ml[kBatch];
+            float ob[kBatch][EPL];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const size_t x = p[min(i + c * kJoinWarps, p.n - 1u)];
+            for (int c = 0; c < kBatch; ++c) {
+                if (i + c * kJoinWarps >= p.n) break;
+                const size_t x = p[i + c * kJoinWarps];
                 ml[c] = mls[x];
 #pragma unroll
                 for (int r = 0; r < EPL; ++r) ob[c][r] = rows[x * HD + lane + 32 * r];
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < kBatch; ++c) {
                 if (i + c * kJoinWarps >= p.n) break;
                 const float top = fmaxf(M, ml[c].x), use = top == -INFINITY ? 0.0f : top;
                 const float al = exp2f(M - use), f = exp2f(ml[c].x - use);  // a warp that saw no row: 0
@@ -510,24 +531,22 @@ __global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(cons
 #pragma unroll
         for (int r = 0; r < EPL; ++r) so[warp][lane + 32 * r] = O[r];
         __syncthreads();
-        if (tid < HD) {
+        for (uint32_t d = tid; d < HD; d += kJoinThreads) {
             float top = sm[0];
 #pragma unroll
-            for (uint32_t w = 1; w < kJoinWarps; ++w) top = fmaxf(top, sm[w]);
+            for (uint32_t x = 1; x < kJoinWarps; ++x) top = fmaxf(top, sm[x]);
             const float use = top == -INFINITY ? 0.0f : top;
             float l = 0.0f, o = 0.0f;
 #pragma unroll
-            for (uint32_t w = 0; w < kJoinWarps; ++w) {
-                const float f = exp2f(sm[w] - use);  // a warp that had no piece: 0
-                l = fmaf(f, sl[w], l);
-                o = fmaf(f, so[w][tid], o);
+            for (uint32_t x = 0; x < kJoinWarps; ++x) {
+                const float f = exp2f(sm[x] - use);  // a warp that had no piece: 0
+                l = fmaf(f, sl[x], l);
+                o = fmaf(f, so[x][d], o);
             }
-            a.out[((size_t)s * a.heads + head) * HD + tid] = o / l;
+            a.out[((size_t)s * a.heads + blockIdx.x) * HD + d] = o / l;
         }
         return;
     }
-    const uint32_t kvh = (blockIdx.x - a.heads) % a.kv_heads, row0 = (blockIdx.x - a.heads) / a.kv_heads * kCountRows;
-    if (row0 > len) return;
     for (uint32_t x = warp; x < a.group; x += kJoinWarps) {  // a head's maximum and sum, a lane a piece
         const pieces p = of(kvh * a.group + x);
         const float2 *mls = p.whole ? a.whole_ml : a.part_ml;
@@ -546,20 +565,23 @@ __global__ void __launch_bounds__(kJoinThreads) attention_paged_join_kernel(cons
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         if (lane == 0) {
             sm[x] = top - kUnit;
-            sl[x] = L;
+            sl[x] = 1.0f / L;
         }
     }
     __syncthreads();
-    const uint32_t start = first_row(len, a.window);
-    const size_t base = ((size_t)s * a.kv_heads + kvh) * a.cap;
-    for (uint32_t j = row0 + tid; j < row0 + kCountRows && j <= len; j += kJoinThreads) {
-        float w = a.w_in && j < len ? a.w_in[base + j] : 0.0f;  // the new row has drawn nothing before
+#pragma unroll
+    for (uint32_t r = 0; r < kCountEach; ++r) {
+        const uint32_t j = row0 + r * kJoinThreads + tid;
+        if (j > len) break;
         if (j >= start) {
             float sum = 0.0f;
-            for (uint32_t h = 0; h < a.group; ++h) sum += exp2f(a.scores[(base + j) * a.group + h] - sm[h]) / sl[h];
-            w += sum;
+#pragma unroll
+            for (uint32_t h = 0; h < 4u; ++h)
+                if (h < a.group) sum = fmaf(exp2f(z[r][h] - sm[h]), sl[h], sum);
+            for (uint32_t h = 4; h < a.group; ++h) sum = fmaf(exp2f(a.scores[(base + j) * a.group + h] - sm[h]), sl[h], sum);
+            w[r] += sum;
         }
-        a.w_out[base + j] = w;
+        a.w_out[base + j] = w[r];
     }
 }
 
@@ -596,10 +618,14 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
     const uint64_t vectors = (uint64_t)a.n_seq * (a.heads + a.kv_heads);
     cudaError_t e = tm_launch_pdl(ctx, attention_paged_vectors_kernel<HD>, dim3((uint32_t)((vectors + 7) / 8)), dim3(256), 0, a);
     if (e == cudaSuccess) e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
-    const uint32_t count = a.w_out ? a.kv_heads * ((a.cap + kCountRows - 1) / kCountRows) : 0u;
-    if (e == cudaSuccess)
-        e = tm_launch_pdl(ctx, attention_paged_join_kernel<HD>, dim3(a.heads + count, a.n_seq), dim3(kJoinThreads), 0, a);
-    return e;
+    if (e != cudaSuccess) return e;
+    // With few heads in all their pieces are many, and CTAs of 16 warps read them at once (one sequence of 131071 rows: 4 us
+    // less); with many heads small CTAs find a place sooner (32 sequences of 1000: 4 us less).
+    const bool few = (uint64_t)a.heads * a.n_seq <= 2u * (uint32_t)ctx->sm_count;
+    const uint32_t rows = kCountEach * 32u * (few ? 16u : 4u), count = a.w_out ? a.kv_heads * ((a.cap + rows - 1) / rows) : 0u;
+    const dim3 grid(a.heads + count, a.n_seq);
+    return few ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 16>, grid, dim3(512), 0, a)
+               : tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 4>, grid, dim3(128), 0, a);
 }
 
 // ---- copies between dense planes and pages ---------------------------------------------------------
@@ -900,6 +926,9 @@ int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_c
     if (kv_stride == 0) kv_stride = kv_heads * head_dim;
     if (q_stride < heads * head_dim || kv_stride < kv_heads * head_dim)
         return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "row strides %u / %u below the row widths", q_stride, kv_stride);
+    if ((uint64_t)n_seq * kv_heads * ((heads / kv_heads + 7u) / 8u) * (((uint64_t)max_pages * page_rows + kTile - 1) / kTile) > 0xffffffffu)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "paged attention: %u sequences of %u KV heads and up to %llu rows", n_seq,
+                       kv_heads, (unsigned long long)max_pages * page_rows);
     const size_t nq = ((size_t)(n_seq - 1) * q_stride + (size_t)heads * head_dim) * 4;
     const size_t nkv = ((size_t)(n_seq - 1) * kv_stride + (size_t)kv_heads * head_dim) * 4;
     const size_t cap = (size_t)max_pages * page_rows, nout = (size_t)n_seq * heads * head_dim * 4;
