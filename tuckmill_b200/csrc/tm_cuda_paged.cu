@@ -171,13 +171,18 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
     const uint32_t kvh = x - a.heads, len = a.len[s], pos = a.pos[s];
     const float *src = is_k ? a.k + (size_t)s * a.kv_stride + (size_t)kvh * HD : a.q + (size_t)s * a.q_stride + (size_t)x * HD;
     const float *nw = is_k ? a.k_norm : a.q_norm, *vs = a.v + (size_t)s * a.kv_stride + (size_t)kvh * HD;
-    float y[EPL], w[EPL], v[EPL], ss = 0.0f;
+    const uint32_t half = a.n_rot / 2u;
+    constexpr int kPairs = HD > 64 ? HD / 64 : 1;  // rotation pairs of a lane, at most
+    float y[EPL], w[EPL], v[EPL], freq[kPairs], ss = 0.0f;
 #pragma unroll
     for (int r = 0; r < EPL; ++r) {
         y[r] = src[lane + 32 * r];
         w[r] = nw[lane + 32 * r];
         v[r] = is_k ? vs[lane + 32 * r] : 0.0f;
     }
+#pragma unroll
+    for (int r = 0; r < kPairs; ++r) freq[r] = lane + 32 * r < half ? a.inv_freq[lane + 32 * r] : 0.0f;
+    const uint32_t id = is_k && len < a.cap ? a.table[(size_t)s * a.max_pages + (len >> a.page_log)] : 0u;
     if (len >= a.cap) {
         if (x == 0u && lane == 0 && len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
         return;
@@ -191,16 +196,19 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
 #pragma unroll
     for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = y[r] * inv * w[r];
     __syncwarp();
-    const uint32_t half = a.n_rot / 2u;
-    for (uint32_t i = lane; i < half; i += 32u) {
-        const float angle = (float)pos * a.inv_freq[i], c = cosf(angle), sn = sinf(angle);
-        const float x0 = row[i], x1 = row[i + half];
-        row[i] = x0 * c - x1 * sn;
-        row[i + half] = x0 * sn + x1 * c;
+#pragma unroll
+    for (int r = 0; r < kPairs; ++r) {
+        const uint32_t i = lane + 32 * r;
+        if (i < half) {
+            float sn, c;
+            sincosf((float)pos * freq[r], &sn, &c);
+            const float x0 = row[i], x1 = row[i + half];
+            row[i] = x0 * c - x1 * sn;
+            row[i + half] = x0 * sn + x1 * c;
+        }
     }
     __syncwarp();
     if (is_k) {
-        const uint32_t id = a.table[(size_t)s * a.max_pages + (len >> a.page_log)];
         if (id >= a.pages) {
             if (lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
             return;
@@ -445,33 +453,34 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Joins the warps' pieces of every pair (a CTA a head, a warp a piece), and counts the attention of stretches of rows (the
-// CTAs behind those).
+// Joins the warps' pieces of every pair (a CTA takes DIMS of a head, a warp a piece), and counts the attention of stretches
+// of rows (the CTAs behind those).  What needs neither pieces nor scores is done while the rows are still being read, and
+// every warp finds the maximum of all pieces for itself, so that nothing waits for it but the last sums.
 constexpr uint32_t kCountEach = 4;
-template <int HD, uint32_t kJoinWarps>
+template <int HD, int DIMS, uint32_t kJoinWarps>
 __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(const paged_args a) {
-    constexpr int EPL = HD / 32, kBatch = 4;
-    constexpr uint32_t kJoinThreads = 32 * kJoinWarps, kCountRows = kCountEach * kJoinThreads;
-    __shared__ float sm[32], sl[32], so[kJoinWarps][HD];
+    constexpr int EPL = DIMS / 32, kBatch = EPL == 1 ? 10 : 2;
+    constexpr uint32_t kParts = HD / DIMS, kJoinThreads = 32 * kJoinWarps, kCountRows = kCountEach * kJoinThreads;
+    __shared__ float sm[32], sl[32], so[kJoinWarps][DIMS];
     tmdev::pdl_trigger();
-    tmdev::pdl_wait();
     const uint32_t s = blockIdx.y, tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u;
-    const uint32_t len = a.len[s], nt = pair_tiles(len, a);
-    if (nt == 0u) return;
-    const bool joins = blockIdx.x < a.heads;
-    const uint32_t kvh = joins ? blockIdx.x / a.group : (blockIdx.x - a.heads) % a.kv_heads;
-    const uint32_t row0 = joins ? 0u : (blockIdx.x - a.heads) / a.kv_heads * kCountRows, start = first_row(len, a.window);
-    if (row0 > len) return;
-    // What the rows have drawn before and the first four heads' scores are asked for before the pieces are known.
+    const uint32_t len = a.len[s], nt = pair_tiles(len, a), joining = a.heads * kParts;
+    const bool joins = blockIdx.x < joining;
+    const uint32_t head = blockIdx.x / kParts, d0 = blockIdx.x % kParts * DIMS;  // (of one that joins)
+    const uint32_t kvh = joins ? head / a.group : (blockIdx.x - joining) % a.kv_heads;
+    const uint32_t row0 = joins ? 0u : (blockIdx.x - joining) / a.kv_heads * kCountRows, start = first_row(len, a.window);
+    if (nt == 0u || row0 > len) {
+        tmdev::pdl_wait();
+        return;
+    }
     const size_t base = ((size_t)s * a.kv_heads + kvh) * a.cap;
-    float w[kCountEach], z[kCountEach][4];
+    float w[kCountEach];
+    __align__(16) float z[kCountEach][4];
     if (!joins) {
 #pragma unroll
         for (uint32_t r = 0; r < kCountEach; ++r) {
             const uint32_t j = row0 + r * kJoinThreads + tid;
             w[r] = a.w_in && j < len ? a.w_in[base + j] : 0.0f;  // the new row has drawn nothing before
-#pragma unroll
-            for (uint32_t h = 0; h < 4u; ++h) z[r][h] = h < a.group && j >= start && j <= len ? a.scores[(base + j) * a.group + h] : 0.0f;
         }
     }
     const uint32_t pairs = a.kv_heads * a.blocks;
@@ -496,56 +505,69 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(c
         return p;
     };
     if (joins) {
-        const pieces p = of(blockIdx.x);
+        const pieces p = of(head);
+        tmdev::pdl_wait();
         const float *rows = p.whole ? a.whole : a.part;
         const float2 *mls = p.whole ? a.whole_ml : a.part_ml;
-        float M = -INFINITY, L = 0.0f, O[EPL];
+        float top = -INFINITY, L = 0.0f, O[EPL];
 #pragma unroll
         for (int r = 0; r < EPL; ++r) O[r] = 0.0f;
-        for (uint32_t i = warp; i < p.n; i += kBatch * kJoinWarps) {
-            float2 ml[kBatch];
-            float ob[kBatch][EPL];
+        float2 ml[kBatch];
+        float ob[kBatch][EPL];
+        auto fetch = [&](uint32_t i) {
 #pragma unroll
             for (int c = 0; c < kBatch; ++c) {
-                if (i + c * kJoinWarps >= p.n) break;
-                const size_t x = p[i + c * kJoinWarps];
-                ml[c] = mls[x];
+                const bool live = i + c * kJoinWarps < p.n;
+                const size_t x = p[live ? i + c * kJoinWarps : 0u];
+                ml[c] = live ? mls[x] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-                for (int r = 0; r < EPL; ++r) ob[c][r] = rows[x * HD + lane + 32 * r];
+                for (int r = 0; r < EPL; ++r) ob[c][r] = live ? rows[x * HD + d0 + lane + 32 * r] : 0.0f;
             }
+        };
+        fetch(warp);
+#pragma unroll 4
+        for (uint32_t i = lane; i < p.n; i += 32u) top = fmaxf(top, mls[p[i]].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float use = top == -INFINITY ? 0.0f : top;
+        for (uint32_t i = warp; i < p.n;) {
 #pragma unroll
             for (int c = 0; c < kBatch; ++c) {
-                if (i + c * kJoinWarps >= p.n) break;
-                const float top = fmaxf(M, ml[c].x), use = top == -INFINITY ? 0.0f : top;
-                const float al = exp2f(M - use), f = exp2f(ml[c].x - use);  // a warp that saw no row: 0
-                M = top;
-                L = fmaf(L, al, f * ml[c].y);
+                const float f = exp2f(ml[c].x - use);  // a warp that saw no row: 0
+                L = fmaf(f, ml[c].y, L);
 #pragma unroll
-                for (int r = 0; r < EPL; ++r) O[r] = fmaf(O[r], al, f * ob[c][r]);
+                for (int r = 0; r < EPL; ++r) O[r] = fmaf(f, ob[c][r], O[r]);
             }
+            i += kBatch * kJoinWarps;
+            if (i < p.n) fetch(i);
         }
-        if (lane == 0) {
-            sm[warp] = M;
-            sl[warp] = L;
-        }
+        if (lane == 0) sl[warp] = L;
 #pragma unroll
         for (int r = 0; r < EPL; ++r) so[warp][lane + 32 * r] = O[r];
         __syncthreads();
-        for (uint32_t d = tid; d < HD; d += kJoinThreads) {
-            float top = sm[0];
-#pragma unroll
-            for (uint32_t x = 1; x < kJoinWarps; ++x) top = fmaxf(top, sm[x]);
-            const float use = top == -INFINITY ? 0.0f : top;
+        for (uint32_t d = tid; d < (uint32_t)DIMS; d += kJoinThreads) {
             float l = 0.0f, o = 0.0f;
 #pragma unroll
             for (uint32_t x = 0; x < kJoinWarps; ++x) {
-                const float f = exp2f(sm[x] - use);  // a warp that had no piece: 0
-                l = fmaf(f, sl[x], l);
-                o = fmaf(f, so[x][d], o);
+                l += sl[x];
+                o += so[x][d];
             }
-            a.out[((size_t)s * a.heads + blockIdx.x) * HD + d] = o / l;
+            a.out[((size_t)s * a.heads + head) * HD + d0 + d] = o / l;
         }
         return;
+    }
+    tmdev::pdl_wait();
+#pragma unroll
+    for (uint32_t r = 0; r < kCountEach; ++r) {
+        const uint32_t j = row0 + r * kJoinThreads + tid;
+        const bool seen = j >= start && j <= len;
+        const float *row = a.scores + (base + j) * a.group;
+        if (a.group % 4u == 0u) {
+            if (seen) *(float4 *)z[r] = *(const float4 *)row;
+        } else {
+#pragma unroll
+            for (uint32_t h = 0; h < 4u; ++h) z[r][h] = seen && h < a.group ? row[h] : 0.0f;
+        }
     }
     for (uint32_t x = warp; x < a.group; x += kJoinWarps) {  // a head's maximum and sum, a lane a piece
         const pieces p = of(kvh * a.group + x);
@@ -612,20 +634,25 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
         if (e != cudaSuccess) return e;
         if (device >= 0 && device < 64) attr_done[device].store(true, std::memory_order_release);
     }
-    const uint64_t tiles = ((uint64_t)a.cap + kTile - 1) / kTile * a.n_seq * a.kv_heads * a.blocks;
+    // At most: tiles of a pair, pairs, and with these the CTAs.
+    const uint32_t whole = (a.cap + kTile - 1) / kTile, seen = a.window ? (a.window + kTile - 2) / kTile + 1u : whole;
+    const uint32_t tiles = seen < whole ? seen : whole, pairs = a.n_seq * a.kv_heads * a.blocks;
     const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), most_ctas(HD));
-    a.ctas = (uint32_t)(tiles < places ? tiles : places);
+    a.ctas = (uint32_t)min((uint64_t)tiles * pairs, (uint64_t)places);
     const uint64_t vectors = (uint64_t)a.n_seq * (a.heads + a.kv_heads);
     cudaError_t e = tm_launch_pdl(ctx, attention_paged_vectors_kernel<HD>, dim3((uint32_t)((vectors + 7) / 8)), dim3(256), 0, a);
     if (e == cudaSuccess) e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
     if (e != cudaSuccess) return e;
-    // With few heads in all their pieces are many, and CTAs of 16 warps read them at once (one sequence of 131071 rows: 4 us
-    // less); with many heads small CTAs find a place sooner (32 sequences of 1000: 4 us less).
-    const bool few = (uint64_t)a.heads * a.n_seq <= 2u * (uint32_t)ctx->sm_count;
-    const uint32_t rows = kCountEach * 32u * (few ? 16u : 4u), count = a.w_out ? a.kv_heads * ((a.cap + rows - 1) / rows) : 0u;
-    const dim3 grid(a.heads + count, a.n_seq);
-    return few ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 16>, grid, dim3(512), 0, a)
-               : tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 4>, grid, dim3(128), 0, a);
+    // The join.  Many heads: a CTA of four warps a head (32 sequences of 1000 rows: 22.4 us, with 16 warps 29.8).  Few: their
+    // dims are cut into CTAs of 32 (8 sequences, window 512, one KV head of 256: 8.6, not cut 10.2), and where a pair may lie
+    // in many pieces 16 warps read them (one of 131071 rows: 93.8, with four 98.2; the window's 36 pieces with 16 10.1).
+    const uint32_t pieces = kAttnWarps * min(tiles, a.ctas / pairs + 2u);
+    const bool few = (uint64_t)a.heads * a.n_seq <= 2u * (uint32_t)ctx->sm_count, deep = few && pieces > 64u;
+    const uint32_t rows = kCountEach * 32u * (deep ? 16u : 4u), count = a.w_out ? a.kv_heads * ((a.cap + rows - 1) / rows) : 0u;
+    const dim3 cut(a.heads * (HD / 32) + count, a.n_seq), uncut(a.heads + count, a.n_seq);
+    return deep  ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 16>, cut, dim3(512), 0, a)
+           : few ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 4>, cut, dim3(128), 0, a)
+                 : tm_launch_pdl(ctx, attention_paged_join_kernel<HD, HD, 4>, uncut, dim3(128), 0, a);
 }
 
 // ---- copies between dense planes and pages ---------------------------------------------------------
