@@ -837,50 +837,117 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const ev
     }
 }
 
-// Moves the kept rows.  In place a CTA takes 64 bytes of every row of a head, so that the columns need not wait for one
-// another, and goes up the rows: what it stores lies at or below what it has read.  Into other pages every stretch of rows
-// is a CTA of its own.
-constexpr uint32_t kMoveThreads = 256, kMoveEach = 8;
-template <int HD, bool IN_PLACE>
-__global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const evict_args a) {
-    constexpr uint32_t kLanes = IN_PLACE ? 4 : HD / 8, kSlices = HD / 8 / kLanes, kRows = kMoveThreads / kLanes * kMoveEach;
+// Moves the kept rows.
+constexpr uint32_t kMoveThreads = 256;
+constexpr uint32_t kNoRow = 0xffffffffu;  // (a pool has fewer rows than that)
+
+// Row j of a head in the pool, as a number of rows from its start.
+__device__ __forceinline__ uint32_t pool_row(const evict_args &a, const uint32_t *pages, uint32_t h, uint32_t j) {
+    const uint32_t id = pages[j >> a.page_log];
+    if (id < a.pages) return ((id * a.kv_heads + h) << a.page_log) + (j & ((1u << a.page_log) - 1u));
+    atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
+    return kNoRow;
+}
+
+// Into other pages: a stretch of rows of a head at a time, keys and values.  A row's place is behind two loads that depend
+// on one another (its number, its page), so each CTA looks two stretches ahead: while the rows of one are on their way, the
+// pages of the next and the numbers of the one after it are too.
+constexpr uint32_t kMoveEach = 4;
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads, 3) kv_evict_move_kernel(const evict_args a, uint32_t n_heads, uint32_t stretches) {
+    constexpr uint32_t kLanes = HD / 8, kPass = kMoveThreads / kLanes, kRows = kPass * kMoveEach;
+    tmdev::pdl_trigger();
+    tmdev::pdl_wait();
+    const uint32_t lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, items = n_heads * stretches;
+    auto rows_of = [&](uint32_t item) -> uint32_t {  // rows of the item's sequence that are kept, 0 behind the last item
+        if (item >= items) return 0u;
+        const uint32_t len = a.len[item / stretches / a.kv_heads];
+        return len > a.cap ? 0u : min(len, a.keep);
+    };
+    auto numbers = [&](uint32_t item, uint32_t n, uint32_t (&j)[kMoveEach]) {
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) {
+            const uint32_t i = item % stretches * kRows + x * kPass + r;
+            j[x] = i < n ? a.kept[(size_t)(item / stretches) * a.keep + i] : kNoRow;
+        }
+    };
+    auto places = [&](uint32_t item, const uint32_t (&j)[kMoveEach], uint32_t (&src)[kMoveEach], uint32_t (&dst)[kMoveEach]) {
+        const uint32_t head = item / stretches, h = head % a.kv_heads;
+        const size_t table = (size_t)(head / a.kv_heads) * a.max_pages;
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) {
+            src[x] = dst[x] = kNoRow;
+            if (j[x] == kNoRow) continue;
+            src[x] = pool_row(a, a.table + table, h, j[x]);
+            dst[x] = pool_row(a, a.to + table, h, item % stretches * kRows + x * kPass + r);
+        }
+    };
+    uint32_t item = blockIdx.x, j[kMoveEach], src[kMoveEach], dst[kMoveEach];
+    numbers(item, rows_of(item), j);
+    places(item, j, src, dst);
+    numbers(item + gridDim.x, rows_of(item + gridDim.x), j);
+    uint32_t ahead = rows_of(item + 2u * gridDim.x);
+    for (; item < items; item += gridDim.x) {
+        uint4 k[kMoveEach], v[kMoveEach];
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) {
+            k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
+            if (src[x] == kNoRow) continue;
+            const size_t at = (size_t)src[x] * HD + lane * 8u;
+            k[x] = *(const uint4 *)(a.kp + at);
+            v[x] = *(const uint4 *)(a.vp + at);
+        }
+        uint32_t to[kMoveEach];
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) to[x] = dst[x];
+        places(item + gridDim.x, j, src, dst);
+        numbers(item + 2u * gridDim.x, ahead, j);
+        ahead = rows_of(item + 3u * gridDim.x);
+#pragma unroll
+        for (uint32_t x = 0; x < kMoveEach; ++x) {
+            if (to[x] == kNoRow) continue;
+            const size_t at = (size_t)to[x] * HD + lane * 8u;
+            *(uint4 *)(a.kp + at) = k[x];
+            *(uint4 *)(a.vp + at) = v[x];
+        }
+    }
+}
+
+// In place: a CTA takes 64 bytes of every row of a head, so that the columns need not wait for one another, and goes up the
+// rows: what it stores lies at or below what it has read.
+constexpr uint32_t kShiftEach = 8, kShiftRows = kMoveThreads / 4 * kShiftEach;
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads) kv_evict_shift_kernel(const evict_args a) {
+    constexpr uint32_t kSlices = HD / 32;
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
     const uint32_t s = blockIdx.y / a.kv_heads, h = blockIdx.y % a.kv_heads, len = a.len[s];
-    if (len > a.cap || (IN_PLACE && len <= a.keep)) return;
-    const uint32_t n = min(len, a.keep);
-    const uint32_t slice = blockIdx.x % kSlices, is_v = blockIdx.x / kSlices % 2u, tile = blockIdx.x / (2u * kSlices);
-    __half *pool = is_v ? a.vp : a.kp;
-    const uint32_t *from = a.table + (size_t)s * a.max_pages, *to = a.to + (size_t)s * a.max_pages;
-    const uint32_t *kept = a.kept + (size_t)blockIdx.y * a.keep;
-    const uint32_t low = (1u << a.page_log) - 1u, lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, col = (slice * kLanes + lane) * 8u;
-    auto place = [&](const uint32_t *pages, uint32_t j) -> __half * {
-        const uint32_t id = pages[j >> a.page_log];
-        if (id >= a.pages) {
-            atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
-            return nullptr;
-        }
-        return pool + ((((size_t)id * a.kv_heads + h) << a.page_log) + (j & low)) * HD + col;
-    };
-    for (uint32_t i0 = tile * kRows; i0 < n; i0 += IN_PLACE ? kRows : n) {
-        uint4 v[kMoveEach];
-        __half *dst[kMoveEach];
+    if (len > a.cap || len <= a.keep) return;
+    __half *pool = blockIdx.x / kSlices ? a.vp : a.kp;
+    const uint32_t *pages = a.table + (size_t)s * a.max_pages, *kept = a.kept + (size_t)blockIdx.y * a.keep;
+    const uint32_t r = threadIdx.x / 4u, col = (blockIdx.x % kSlices * 4u + threadIdx.x % 4u) * 8u;
+    for (uint32_t i0 = 0; i0 < a.keep; i0 += kShiftRows) {
+        uint4 v[kShiftEach];
+        uint32_t dst[kShiftEach];
 #pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) {
-            const uint32_t i = i0 + x * (kMoveThreads / kLanes) + r;
-            dst[x] = nullptr;
-            if (i >= n) continue;
-            const __half *src = place(from, kept[i]);
-            dst[x] = place(to, i);
-            v[x] = src ? *(const uint4 *)src : make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t x = 0; x < kShiftEach; ++x) {
+            const uint32_t i = i0 + x * (kMoveThreads / 4) + r;
+            dst[x] = kNoRow;
+            if (i >= a.keep) continue;
+            const uint32_t j = kept[i];
+            if (j == i) continue;  // it stays where it is
+            const uint32_t src = pool_row(a, pages, h, j);
+            dst[x] = pool_row(a, pages, h, i);
+            v[x] = src != kNoRow ? *(const uint4 *)(pool + (size_t)src * HD + col) : make_uint4(0u, 0u, 0u, 0u);
         }
-        if (IN_PLACE) __syncthreads();  // the whole stretch is read
+        __syncthreads();  // the whole stretch is read
 #pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x)
-            if (dst[x]) *(uint4 *)dst[x] = v[x];
-        if (IN_PLACE) __syncthreads();  // and written before the next is read
+        for (uint32_t x = 0; x < kShiftEach; ++x)
+            if (dst[x] != kNoRow) *(uint4 *)(pool + (size_t)dst[x] * HD + col) = v[x];
+        __syncthreads();  // and written before the next is read
     }
 }
+
 // The lengths, where they replace the ones that both launches above read.
 __global__ void kv_evict_lengths_kernel(uint32_t *len, uint32_t n_seq, uint32_t keep, uint32_t cap) {
     tmdev::pdl_trigger();
@@ -891,11 +958,12 @@ __global__ void kv_evict_lengths_kernel(uint32_t *len, uint32_t n_seq, uint32_t 
 
 template <int HD>
 cudaError_t launch_move(tm_cuda_ctx *ctx, const evict_args &a, uint32_t n_seq, bool in_place) {
-    const uint32_t rows = kMoveThreads / (HD / 8) * kMoveEach, most = a.keep < a.cap ? a.keep : a.cap;
     if (in_place)
-        return tm_launch_pdl(ctx, kv_evict_move_kernel<HD, true>, dim3(2 * (HD / 32), n_seq * a.kv_heads), dim3(kMoveThreads), 0, a);
-    return tm_launch_pdl(ctx, kv_evict_move_kernel<HD, false>, dim3(2 * ((most + rows - 1) / rows), n_seq * a.kv_heads),
-                         dim3(kMoveThreads), 0, a);
+        return tm_launch_pdl(ctx, kv_evict_shift_kernel<HD>, dim3(2 * (HD / 32), n_seq * a.kv_heads), dim3(kMoveThreads), 0, a);
+    const uint32_t rows = kMoveThreads / (HD / 8) * kMoveEach, stretches = (a.keep + rows - 1) / rows, heads = n_seq * a.kv_heads;
+    const uint32_t places = 3u * (uint32_t)ctx->sm_count;
+    const uint32_t ctas = (uint64_t)heads * stretches < places ? heads * stretches : places;
+    return tm_launch_pdl(ctx, kv_evict_move_kernel<HD>, dim3(ctas), dim3(kMoveThreads), 0, a, heads, stretches);
 }
 
 template <int HD>
@@ -1112,6 +1180,8 @@ int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_bu
     if (keep == 0 || keep > cap || (uint64_t)first + recent > keep)
         return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: keep %u of at most %zu rows, the first %u and the last %u among them",
                        keep, cap, first, recent);
+    if ((uint64_t)n_seq * kv_heads * keep > 0x7fffffffu)
+        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: %u rows of %u sequences of %u KV heads", keep, n_seq, kv_heads);
     const size_t nw = (size_t)n_seq * kv_heads * cap * 4, nk = (size_t)n_seq * kv_heads * keep * 4;
     const size_t ntable = (size_t)n_seq * max_pages * 4, nlen = (size_t)n_seq * 4;
     TM_CHECK_BUF(k_pages, pool_bytes(shape), "K pages");
