@@ -435,6 +435,8 @@ EVICT = [
     ([1500, 1400, 800], 2, 128, 64, 700, 0, 0),
     ([300, 0, 257], 1, 256, 256, 256, 3, 100),
     ([5000], 2, 64, 128, 2100, 4, 64),
+    ([9000, 4096, 4097, 3000], 1, 32, 256, 2500, 1, 70),  # on both sides of what registers hold
+    ([3000], 1, 32, 64, 1500, 0, 0),
 ]
 
 

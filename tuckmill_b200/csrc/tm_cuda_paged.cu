@@ -712,10 +712,11 @@ __global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const copy_
 // ---- eviction --------------------------------------------------------------------------------------
 //
 // Per (sequence, KV head): the first `first` rows, the last `recent` rows, and of those between the ones with the largest
-// weights, `keep` in all, in their order.  One CTA finds the smallest weight that stays by three counting passes over
-// 11, 11 and 10 bits of the weights' order-preserving integers (1024 threads, the weights come from L2 after the first),
-// then writes the list of rows; a second launch moves the rows.  What bounds it: the rows' bytes, 8 head_dim each.
-constexpr uint32_t kEvictThreads = 1024;
+// weights, `keep` in all, in their order.  One CTA finds the smallest weight that stays by counting passes over 11, 11 and
+// 10 bits of the weights' order-preserving integers, then lists the rows; a second launch moves them.  Each thread looks
+// after a strip of consecutive rows, whose weights it holds in registers up to 4096 rows.  What bounds it: the rows' bytes,
+// 8 head_dim each.
+constexpr uint32_t kEvictThreads = 512;
 
 struct evict_args {
     __half *kp, *vp;
@@ -733,6 +734,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     const uint32_t b = __float_as_uint(w + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+static_assert(kEvictThreads * 4 == 2048, "four bins a thread");
 // Exclusive prefix sum over the CTA's threads, and the total.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warps, uint32_t &total) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -745,7 +747,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warps, uint
     __syncthreads();
     if (lane == 31u) warps[warp] = incl;
     __syncthreads();
-    uint32_t w = warps[lane], sum = w;  // 32 warps
+    uint32_t w = lane < kEvictThreads / 32u ? warps[lane] : 0u, sum = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -755,8 +757,96 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warps, uint
     return __shfl_sync(0xffffffffu, sum - w, warp) + incl - v;
 }
 
+constexpr uint32_t kHeld = 8;  // weights of a strip in registers
+template <bool HELD>
+__device__ __forceinline__ void select_rows(const evict_args &a, const float *w, float *w_out, uint32_t *kept, uint32_t len, uint32_t (&hist)[2048],
+                                            uint32_t (&warps)[32], uint32_t (&found)[3]) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
+    const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
+    const uint32_t strip = (len + kEvictThreads - 1u) / kEvictThreads, j0 = tid * strip;
+    float held[HELD ? kHeld : 1];
+    if (HELD) {
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e) held[HELD ? e : 0] = e < strip && j0 + e < len ? w[j0 + e] : 0.0f;
+    }
+    // f(row, weight) for the strip's rows
+    auto rows = [&](auto f) {
+        if (HELD) {
+#pragma unroll
+            for (uint32_t e = 0; e < kHeld; ++e)
+                if (e < strip) f(j0 + e, held[HELD ? e : 0]);
+        } else {
+            for (uint32_t e = 0; e < strip; ++e) f(j0 + e, j0 + e < len ? w[j0 + e] : 0.0f);
+        }
+    };
+    // The want-th largest key between lo and hi, digit by digit: `prefix` its bits so far (those of `mask`), `left` how many
+    // are still wanted among the keys that begin with them.
+    uint32_t prefix = 0u, mask = 0u, left = want;
+    if (want > 0u) {
+        const uint32_t shift[3] = {21u, 10u, 0u}, width[3] = {11u, 11u, 10u};
+#pragma unroll 1
+        for (int p = 0; p < 3; ++p) {
+            *(uint4 *)(hist + 4u * tid) = make_uint4(0u, 0u, 0u, 0u);
+            __syncthreads();
+            const uint32_t digits = (1u << width[p]) - 1u;
+            rows([&](uint32_t j, float v) {
+                const uint32_t key = weight_key(v);
+                const bool mine = j >= lo && j < hi && (key & mask) == prefix;
+                // rows that nothing has looked at tie: a warp counts its zeros at once
+                const uint32_t zeros = __ballot_sync(0xffffffffu, mine && key == 0x80000000u);
+                if (mine && (key != 0x80000000u || lane == (uint32_t)__ffs(zeros) - 1u))
+                    atomicAdd(&hist[(key >> shift[p]) & digits], key != 0x80000000u ? 1u : (uint32_t)__popc(zeros));
+            });
+            __syncthreads();
+            // Thread i: four bins from 2047 - 4i down, so that a prefix sum counts from the top.
+            const uint32_t b = 2044u - 4u * tid;
+            const uint4 c = *(const uint4 *)(hist + b);
+            uint32_t total, above = block_scan(c.x + c.y + c.z + c.w, warps, total);
+            const uint32_t of[4] = {c.w, c.z, c.y, c.x};
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; ++x) {
+                if (above < left && above + of[x] >= left) {
+                    found[0] = b + 3u - x;
+                    found[1] = left - above;
+                    found[2] = of[x];
+                }
+                above += of[x];
+            }
+            __syncthreads();
+            prefix |= found[0] << shift[p];
+            mask |= digits << shift[p];
+            left = found[1];
+            if (found[2] == left) break;  // all that begin with these bits stay
+            __syncthreads();
+        }
+    }
+    // The rows that stay: keys above the border, and the first `left` at it.
+    uint32_t equal = 0u, total;
+    auto middle = [&](uint32_t j) { return j >= lo && j < hi; };
+    if (want > 0u) rows([&](uint32_t j, float v) { equal += middle(j) && (weight_key(v) & mask) == prefix ? 1u : 0u; });
+    const uint32_t eq = block_scan(equal, warps, total);
+    uint32_t e = eq;
+    auto stays = [&](uint32_t j, float v) {
+        if (j >= len) return false;
+        if (!middle(j)) return true;
+        if (want == 0u) return false;
+        const uint32_t key = weight_key(v) & mask;
+        return key > prefix || (key == prefix && e++ < left);
+    };
+    uint32_t mine = 0u;
+    rows([&](uint32_t j, float v) { mine += stays(j, v) ? 1u : 0u; });
+    uint32_t at = block_scan(mine, warps, total);  // (behind its barriers all weights that are held have been read)
+    e = eq;
+    rows([&](uint32_t j, float v) {
+        if (!stays(j, v)) return;
+        if (HELD) w_out[at] = v;
+        kept[at++] = j;
+    });
+}
+
 __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const evict_args a) {
-    __shared__ uint32_t hist[2048], warps[32], found[2];
+    __shared__ __align__(16) uint32_t hist[2048];
+    __shared__ uint32_t warps[32], found[3];
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
     const uint32_t s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, len = a.len[s];
@@ -770,64 +860,23 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const ev
     if (a.len_out && h == 0 && tid == 0) a.len_out[s] = min(len, a.keep);
     const size_t head = (size_t)s * a.kv_heads + h;
     const float *w = a.w + head * a.cap;
+    float *w_out = a.w_out + head * a.cap;
     uint32_t *kept = a.kept + head * a.keep;
     const uint32_t n = min(len, a.keep);
     if (len <= a.keep) {
-        for (uint32_t i = tid; i < a.keep; i += kEvictThreads) kept[i] = i < len ? i : TM_CUDA_SEQ_NONE;
-    } else {
-        const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
-        // The want-th largest key between lo and hi, digit by digit: `prefix` its bits so far, `left` how many are
-        // still wanted among the keys that begin with them.
-        uint32_t prefix = 0u, left = want;
-        const uint32_t shift[3] = {21u, 10u, 0u}, width[3] = {11u, 11u, 10u};
-        if (want > 0u) {
-#pragma unroll 1
-            for (int p = 0; p < 3; ++p) {
-                for (uint32_t b = tid; b < 2048u; b += kEvictThreads) hist[b] = 0u;
-                __syncthreads();
-                const uint32_t mask = p == 0 ? 0u : ~0u << (shift[p] + width[p]);
-                for (uint32_t j = lo + tid; j < hi; j += kEvictThreads) {
-                    const uint32_t key = weight_key(w[j]);
-                    if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift[p]) & ((1u << width[p]) - 1u)], 1u);
-                }
-                __syncthreads();
-                // Thread i: bins 2047 - 2i and below it, so that a prefix sum counts from the top.
-                const uint32_t b1 = 2047u - 2u * tid, c1 = hist[b1], c0 = hist[b1 - 1u];
-                uint32_t total;
-                const uint32_t above = block_scan(c1 + c0, warps, total);
-                if (above < left && above + c1 + c0 >= left) {
-                    const bool upper = above + c1 >= left;
-                    found[0] = upper ? b1 : b1 - 1u;
-                    found[1] = left - above - (upper ? 0u : c1);
-                }
-                __syncthreads();
-                prefix |= found[0] << shift[p];
-                left = found[1];
-                __syncthreads();
-            }
+        for (uint32_t i = tid; i < a.keep; i += kEvictThreads) {
+            kept[i] = i < len ? i : TM_CUDA_SEQ_NONE;
+            if (i < len && w_out != w) w_out[i] = w[i];
         }
-        // Each thread lists a contiguous strip of rows: keys above the border, and the first `left` equal to it.
-        const uint32_t strip = (len + kEvictThreads - 1u) / kEvictThreads, j0 = min(len, tid * strip), j1 = min(len, j0 + strip);
-        uint32_t equal = 0u, total;
-        if (want > 0u)
-            for (uint32_t j = max(j0, lo); j < min(j1, hi); ++j) equal += weight_key(w[j]) == prefix ? 1u : 0u;
-        uint32_t eq = block_scan(equal, warps, total);
-        auto stays = [&](uint32_t j, uint32_t &e) {
-            if (j < lo || j >= hi) return true;
-            if (want == 0u) return false;
-            const uint32_t key = weight_key(w[j]);
-            return key > prefix || (key == prefix && e++ < left);
-        };
-        uint32_t mine = 0u, e = eq;
-        for (uint32_t j = j0; j < j1; ++j) mine += stays(j, e) ? 1u : 0u;
-        uint32_t at = block_scan(mine, warps, total);
-        e = eq;
-        for (uint32_t j = j0; j < j1; ++j)
-            if (stays(j, e)) kept[at++] = j;
+        return;
     }
+    if (len <= kHeld * kEvictThreads) {
+        select_rows<true>(a, w, w_out, kept, len, hist, warps, found);
+        return;
+    }
+    select_rows<false>(a, w, w_out, kept, len, hist, warps, found);
     __syncthreads();
     // The weights go with their rows.  A row never moves up, so reading a stretch before it is written is enough in place.
-    float *w_out = a.w_out + head * a.cap;
     for (uint32_t i0 = 0; i0 < n; i0 += kEvictThreads) {
         const uint32_t i = i0 + tid;
         const float v = i < n ? w[kept[i]] : 0.0f;
@@ -852,9 +901,9 @@ __device__ __forceinline__ uint32_t pool_row(const evict_args &a, const uint32_t
 // Into other pages: a stretch of rows of a head at a time, keys and values.  A row's place is behind two loads that depend
 // on one another (its number, its page), so each CTA looks two stretches ahead: while the rows of one are on their way, the
 // pages of the next and the numbers of the one after it are too.
-constexpr uint32_t kMoveEach = 4;
+constexpr uint32_t kMoveEach = 2;
 template <int HD>
-__global__ void __launch_bounds__(kMoveThreads, 3) kv_evict_move_kernel(const evict_args a, uint32_t n_heads, uint32_t stretches) {
+__global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const evict_args a, uint32_t n_heads, uint32_t stretches) {
     constexpr uint32_t kLanes = HD / 8, kPass = kMoveThreads / kLanes, kRows = kPass * kMoveEach;
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
@@ -961,7 +1010,7 @@ cudaError_t launch_move(tm_cuda_ctx *ctx, const evict_args &a, uint32_t n_seq, b
     if (in_place)
         return tm_launch_pdl(ctx, kv_evict_shift_kernel<HD>, dim3(2 * (HD / 32), n_seq * a.kv_heads), dim3(kMoveThreads), 0, a);
     const uint32_t rows = kMoveThreads / (HD / 8) * kMoveEach, stretches = (a.keep + rows - 1) / rows, heads = n_seq * a.kv_heads;
-    const uint32_t places = 3u * (uint32_t)ctx->sm_count;
+    const uint32_t places = 4u * (uint32_t)ctx->sm_count;
     const uint32_t ctas = (uint64_t)heads * stretches < places ? heads * stretches : places;
     return tm_launch_pdl(ctx, kv_evict_move_kernel<HD>, dim3(ctas), dim3(kMoveThreads), 0, a, heads, stretches);
 }
