@@ -5,7 +5,7 @@
 // whose per-token words fit in shared memory, so nothing the size of the vocabulary is kept between calls or cleared: the
 // CTA reads the row's whole log and bias map (a few kilobytes that the row's CTAs share in L2) and counts the tokens of its
 // own stretch with integer atomics, whose order does not matter, while its logits are on their way into registers.  The
-// arithmetic is done once for each named token, by the thread that holds it; all other logits pass from registers to memory
+// arithmetic is done once for each named token; all other logits pass from registers to memory
 // under the mask (words tested for every logit: 32 rows of 151936 34 us instead of 16.7; the log read once by a cluster of
 // CTAs that send each other its entries: 19.4).  Each step is rounded to f32 by itself, so a choice does not hang on how an
 // expression was contracted.
@@ -56,6 +56,7 @@ __device__ __forceinline__ unsigned long long warp_best(float v, uint32_t at) {
 template <int EACH>
 __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_kernel(const logits_args a) {
     constexpr uint32_t kChunk = EACH * 4u * kThreads, kBatch = 8;
+    constexpr int kHalf = EACH > 4 ? 4 : EACH;  // quads that are on their way while the log is counted
     // Of each token: how often the log holds it from the prompt's end on, and above those bits its last bias entry, from 1.
     __shared__ __align__(16) uint32_t words[kChunk];
     __shared__ uint32_t logged[kChunk / 32], biased[kChunk / 32];  // a bit a token: the log holds it; the bias map names it
@@ -75,8 +76,7 @@ __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_ker
     const uint32_t n_bias = a.bias_ids ? min(a.bias_count[r], a.bias_cap) : 0u;
     float v[EACH][4];
     uint32_t allowed = 0u;  // a bit a logit of this thread: the mask lets it through
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
+    auto fetch = [&](int e) {
         const uint32_t i = (e * kThreads + tid) * 4u;
         if (a.quads) {
             if (i < m) *(float4 *)v[e] = *(const float4 *)(x + i);
@@ -84,7 +84,9 @@ __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_ker
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[e][k] = i + k < m ? x[i + k] : 0.0f;
         }
-    }
+    };
+#pragma unroll
+    for (int e = 0; e < kHalf; ++e) fetch(e);
     const bool any = a.penalties || a.bias_ids;
     if (any) {
         for (uint32_t i = tid * 4u; i < kChunk; i += kThreads * 4u) *(uint4 *)(words + i) = make_uint4(0u, 0u, 0u, 0u);
@@ -122,6 +124,8 @@ __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_ker
         }
         __syncthreads();
     }
+#pragma unroll
+    for (int e = kHalf; e < EACH; ++e) fetch(e);
     // ---- the logits that nothing names; the others are stored as they are ----
     float best = -INFINITY;
     // The best's quad; a bit a logit of this thread: a candidate here, named.
@@ -161,20 +165,13 @@ __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_ker
             for (int k = 3; k >= 0; --k)
                 if (v[e][k] == best && (mine >> (4 * e + k) & 1u) != 0u && (!found || best_quad == e)) best_at = c0 + (e * kThreads + tid) * 4u + k;
     }
-    // ---- the others, by the thread that holds them ----
+    // ---- the others ----
     const float repetition = a.penalties ? a.penalties[r * 3] : 1.0f, presence = a.penalties ? a.penalties[r * 3 + 1] : 0.0f;
     const float frequency = a.penalties ? a.penalties[r * 3 + 2] : 0.0f;
 #pragma unroll 1
     for (; others != 0u; others &= others - 1u) {
         const uint32_t j = __ffs(others) - 1u, at = ((j >> 2) * kThreads + tid) * 4u + (j & 3u);
-        float tree[EACH * 4];
-#pragma unroll
-        for (int i = 0; i < EACH * 4; ++i) tree[i] = v[i / 4][i % 4];
-#pragma unroll
-        for (int half = EACH * 2; half > 0; half >>= 1)
-#pragma unroll
-            for (int i = 0; i < half; ++i) tree[i] = j & half ? tree[i + half] : tree[i];
-        float z = tree[0];
+        float z = x[at];  // (this thread has stored it as it was, if y is x)
         const uint32_t word = words[at], count = word & ((1u << kCountBits) - 1u), entry = word >> kCountBits;
         const float bias = entry != 0u ? a.bias_values[(size_t)r * a.bias_cap + entry - 1u] : 0.0f;
         if (logged[at / 32u] >> (at & 31u) & 1u) {
