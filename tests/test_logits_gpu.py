@@ -44,6 +44,11 @@ CASES = [
     (33, 32001, 90, 3, True, 0),
     (1, 151936, 3000, 300, True, 1),
     (1, 600001, 100, 10, False, 0),
+    (70, 32000, 9, 2, True, 0),     # stretches of 4096 logits, rows in quads
+    (70, 32001, 9, 2, True, 0),     # and not
+    (150, 32004, 5, 1, True, 0),    # stretches of 8192
+    (150, 32003, 5, 0, False, 0),
+    (1, cuda.LOGITS_MAX, 50, 4, True, 0),
 ]
 
 

@@ -175,6 +175,11 @@ CASES = [
     ([40, 41], 17, 1, 32, 16, {}),
     ([i * 7 % 130 for i in range(70)], 4, 4, 64, 16, {}),
     ([20, NONE, 33], 4, 2, 128, 16, {}),
+    # many heads in all: the join's uncut form, at every head size
+    ([(i * 37) % 200 for i in range(40)], 8, 2, 128, 32, {}),
+    ([(i * 53) % 150 for i in range(40)], 8, 1, 256, 16, {"window": 70}),
+    ([(i * 11) % 90 for i in range(80)], 4, 4, 32, 16, {}),
+    ([(i * 29) % 300 for i in range(160)], 2, 2, 64, 64, {"dropped": 5}),
 ]
 
 
@@ -251,7 +256,7 @@ def test_a_full_sequence_and_a_bad_page(ctx):
     t.bk.upload(gone * t.k[0].nbytes, t.k[gone])
     t.bv.upload(gone * t.v[0].nbytes, t.v[gone])
     t.check()
-    # the new row's own page is not there: nothing is stored, the token still sees itself
+    # the new row's own page is not there: nothing is stored, the row is zeros like the page's others
     t = Paged(ctx, [17], 2, 2, 64, 16, seed=9)
     page = t.table[0, 1]
     t.k[page, :, 0] = t.v[page, :, 0] = 0
@@ -262,9 +267,14 @@ def test_a_full_sequence_and_a_bad_page(ctx):
     ctx.fence()
     assert status_of(t.status) == cuda.STATUS_BAD_PAGE
     np.testing.assert_array_equal(f16(t.bk, t.k.shape).view(np.uint16), t.k.view(np.uint16))
-    x = t.qkv[0].reshape(-1, 64)
+    t.k[page], t.v[page] = 0, 0  # keys of zeros weigh exp(0) each
     out = f32(t.bout, (2, 64))
-    assert np.all(np.isfinite(out)) and not np.allclose(out, x[4:6], atol=1e-3)
+    q, qmag = t.turned(t.qkv[0].reshape(-1, 64)[:2], t.qn, t.pos[0])
+    for h in range(2):
+        keys, vals = [np.concatenate([x[t.table[0, 0], h], x[page, h, :2]]).astype(np.float64) for x in (t.k, t.v)]
+        p = np.exp(keys @ q[h] * float(t.scale))
+        Z = float(t.scale) * (np.abs(keys) @ qmag[h]).max()
+        assert np.all(np.abs(out[h] - p @ vals / p.sum()) <= (100 * Z + 82) * U * (p @ np.abs(vals) / p.sum()))
 
 
 def test_a_recorded_step_grows_its_sequences(ctx):
@@ -335,6 +345,160 @@ def test_attention_refusals(ctx):
         assert e.value.code in (-4, -5), over
     t.call(w_out=w)
     ctx.fence()
+
+
+def test_a_pool_past_four_gigabytes(ctx):
+    """Pages whose byte offsets pass 32 bits: what is stored, read, copied and moved there is what lies there."""
+    heads, kvh, hd, page, pages, n = 4, 1, 256, 256, 33000, 300
+    big = [ctx.buffer(pages * kvh * page * hd * 2) for _ in range(2)]
+    size = kvh * page * hd * 2
+    t = Paged(ctx, [n], heads, kvh, hd, page, seed=31, weights=True)
+    ids = np.array([[32999, 32800, 5]], np.uint32)[:, :t.max_pages]
+    for b, x in zip(big, (t.k, t.v)):
+        for j in range(2):
+            b.upload(int(ids[0, j]) * size, x[t.table[0, j]])
+    table = ctx.from_array(ids)
+    w = ctx.from_array(t.w_in)
+    t.call(w, w, k_pages=big[0], v_pages=big[1], table=table, pages=pages)
+    ctx.fence()
+    for b, own in zip(big, (t.bk, t.bv)):  # the small pool gets what the large one holds now
+        for j in range(2):
+            own.upload(int(t.table[0, j]) * size, b.download(int(ids[0, j]) * size, size))
+    t.check(t.w_in, f32(w, t.w_in.shape), t.w_in)
+    # out to a dense plane, and back into other high pages
+    dense = [ctx.buffer(kvh * 512 * hd * 2) for _ in range(2)]
+    high = ctx.from_array(np.array([[32998, 32000, 7]], np.uint32)[:, :t.max_pages])
+    for tb, to_pages in ((table, False), (high, True)):
+        ctx.kv_pages_copy(dense[0], dense[1], big[0], big[1], tb, t.status, pages, page, t.max_pages, kvh, hd, 512, to_pages,
+                          [(0, 0, 0, n)])
+    ctx.fence()
+    for b in big:
+        np.testing.assert_array_equal(b.download(32998 * size, size), b.download(32999 * size, size))
+        np.testing.assert_array_equal(b.download(32000 * size, (n - page) * hd * 2), b.download(32800 * size, (n - page) * hd * 2))
+    kept, length = ctx.buffer(kvh * 40 * 4), ctx.from_array(np.array([n], np.uint32))
+    before = [b.download(int(i) * size, size, np.uint16).reshape(page, hd) for b in big for i in ids[0, :2]]
+    total = f32(w, t.w_in.shape).copy()
+    ctx.kv_pages_evict(big[0], big[1], table, high, length, length, w, w, kept, t.status, 1, kvh, hd, pages, page, t.max_pages,
+                       40, 2, 3)
+    ctx.fence()
+    rows = evicted([n], total, 40, 2, 3)[0, 0]
+    np.testing.assert_array_equal(u32(kept, (40,)), rows)
+    for x, b in enumerate(big):
+        whole = np.concatenate(before[2 * x:2 * x + 2])
+        np.testing.assert_array_equal(b.download(32998 * size, 40 * hd * 2, np.uint16).reshape(40, hd), whole[rows])
+    assert status_of(t.status) == 0
+
+
+def test_as_many_sequences_as_a_call_takes(ctx):
+    """1024 short sequences, most of them absent."""
+    g = np.random.default_rng(5)
+    lens = [NONE if i % 3 else int(g.integers(0, 40)) for i in range(1024)]
+    t = Paged(ctx, lens, 2, 1, 64, 16, seed=41)
+    t.call()
+    ctx.fence()
+    assert status_of(t.status) == 0
+    t.check()
+
+
+def test_operands_that_are_views(ctx):
+    """Every operand a view 16 bytes into a larger buffer."""
+    t = Paged(ctx, [70, 3, 200], 6, 2, 64, 16, weights=True, seed=51)
+
+    def inside(b):
+        whole = ctx.buffer(len(b) + 48)
+        v = whole.view(16, len(b))
+        v.upload(0, b.download(0, len(b)))
+        return v
+
+    names = dict(k_pages="bk", v_pages="bv", table="btable", out="bout", pos_buf="bpos", len_buf="blen", q_norm="bqn", k_norm="bkn",
+                 inv_freq="binv")
+    for n in names.values():
+        setattr(t, n, inside(getattr(t, n)))
+    w = inside(ctx.from_array(t.w_in))
+    t.scratch = ctx.buffer(len(t.scratch) + 16).view(16, len(t.scratch))
+    t.call(w, w)
+    ctx.fence()
+    t.check(t.w_in, f32(w, t.w_in.shape), t.w_in)
+
+
+def steps(ctx, how):
+    """A prompt into its pages, two tokens, an eviction in place, another token and its choice: one operator after the other,
+    each reading what the one before it has just written."""
+    t = Paged(ctx, [40, 25], 8, 2, 64, 16, weights=True, max_pages=6, seed=61)
+    g = np.random.default_rng(61)
+    spare = [p for p in range(t.pages) if p not in t.table]
+    t.table[0, 3:5], t.table[1, 2] = t.table[0, 2], spare[0]
+    table = np.arange(12, dtype=np.uint32).reshape(2, 6)
+    pool = np.zeros((12, 2, 16, 64), np.float16)
+    k, v = ctx.from_array(pool), ctx.from_array(pool)
+    dense = [ctx.from_array(g.standard_normal((2, 2, 48, 64)).astype(np.float16)) for _ in range(2)]
+    btable, blen, bpos = ctx.from_array(np.full((2, 6), 99, np.uint32)), ctx.from_array(np.zeros(2, np.uint32)), ctx.from_array(np.zeros(2, np.uint32))
+    w, kept = ctx.from_array(np.zeros((2, 2, 96), np.float32)), ctx.buffer(2 * 2 * 20 * 4)
+    scratch = ctx.buffer(cuda.attention_paged_scratch_bytes(2, 8, 2, 64, 16, 6, True))
+    log, spot = ctx.from_array(np.zeros((2, 8), np.uint32)), ctx.from_array(np.zeros(2, np.uint32))
+    partial, pen = ctx.buffer(2 * cuda.LOGITS_PARTIAL_BYTES), ctx.from_array(np.array([[1.5, 0.1, 0.2]] * 2, np.float32))
+    y = ctx.buffer(2 * 512 * 4)
+    y.zero()
+    ctx.fence()
+    attend = dict(k_pages=k, v_pages=v, table=btable, len_buf=blen, pos_buf=bpos, scratch=scratch, pages=12, max_pages=6)
+
+    def ops():
+        yield lambda: btable.store_u32(table.reshape(-1))
+        yield lambda: ctx.kv_pages_copy(dense[0], dense[1], k, v, btable, t.status, 12, 16, 6, 2, 64, 48, True, [(0, 0, 0, 40), (1, 1, 0, 25)])
+        yield lambda: blen.store_u32([40, 25])
+        yield lambda: bpos.store_u32([40, 25])
+        for i in range(2):
+            yield lambda: t.call(w, w, **attend)
+            for b in (blen, bpos):
+                yield lambda b=b: ctx.u32_add_sat(b, 0, 2, 1, 95)
+        yield lambda: ctx.kv_pages_evict(k, v, btable, btable, blen, blen, w, w, kept, t.status, 2, 2, 64, 12, 16, 6, 20, 2, 4)
+        yield lambda: t.call(w, w, **attend)
+        yield lambda: ctx.logits_adjust_rows(t.bout, y, 2, 512, log, 8, 0, spot, pen, partial=partial)
+        yield lambda: ctx.u32_add_sat(spot, 0, 2, 1, 7)
+        yield lambda: ctx.logits_adjust_rows(y, y, 2, 512, log, 8, 0, spot, pen, partial=partial)
+
+    if how in ("group", "burst"):
+        ctx._call("begin_" + how)
+    for op in ops():
+        op()
+        if how == "fence":
+            ctx.fence()
+    if how in ("group", "burst"):
+        ctx._call("end_" + how)
+    ctx.fence()
+    return [k, v, w, kept, blen, t.bout, y, log, t.status]
+
+
+def test_operators_one_after_the_other_see_each_others_results(ctx):
+    alone = [b.download(0, len(b)) for b in steps(ctx, "fence")]
+    assert int(alone[-1].view(np.uint32)[0]) == 0
+    for how in ("queued", "group", "burst"):
+        for x, b in zip(alone, steps(ctx, how)):
+            np.testing.assert_array_equal(b.download(0, len(b)), x, err_msg=how)
+
+
+def test_two_contexts_at_once(ctx):
+    """A second context's calls on the same device, neither waiting for the other."""
+    other = cuda.CudaContext(0)
+    try:
+        cases = [Paged(c, [900, 50, 333], 8, 2, 128, 32, weights=True, seed=71) for c in (ctx, other)]
+        ws = [c.ctx.from_array(c.w_in) for c in cases]
+        for c in cases:
+            c.ctx.fence()
+        for _ in range(5):
+            for c, w in zip(cases, ws):
+                c.call(w, w)
+        for c in cases:
+            c.ctx.fence()
+        for a, b in ((cases[0].bout, cases[1].bout), (cases[0].bk, cases[1].bk), (ws[0], ws[1])):
+            np.testing.assert_array_equal(a.download(0, len(a)), b.download(0, len(b)))
+        with pytest.raises(cuda.CudaError):  # one context's buffer in another's call
+            cases[0].call(out=cases[1].bout)
+        del cases, ws, a, b, c, w
+    finally:
+        import gc
+        gc.collect()
+        other.close()
 
 
 # ---------------------------------------------------------------- copies
