@@ -898,68 +898,39 @@ __device__ __forceinline__ uint32_t pool_row(const evict_args &a, const uint32_t
     return kNoRow;
 }
 
-// Into other pages: a stretch of rows of a head at a time, keys and values.  A row's place is behind two loads that depend
-// on one another (its number, its page), so each CTA looks two stretches ahead: while the rows of one are on their way, the
-// pages of the next and the numbers of the one after it are too.
-constexpr uint32_t kMoveEach = 2;
+// Into other pages: a CTA takes 16 KB of a head's rows, keys or values.  A row's place is behind two loads that depend on one
+// another (its number, its page): a thread a row looks them up, then all copy as in kv_pages_copy_kernel.  Many small CTAs
+// hide that better than few that look ahead (32 sequences of 4096 rows, half of them kept: X us instead of 93).
 template <int HD>
-__global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const evict_args a, uint32_t n_heads, uint32_t stretches) {
-    constexpr uint32_t kLanes = HD / 8, kPass = kMoveThreads / kLanes, kRows = kPass * kMoveEach;
+constexpr uint32_t kRowsMoved = 8192u / HD;
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const evict_args a) {
+    constexpr uint32_t kMoveRows = kRowsMoved<HD>, kChunks = HD / 8, kEach = kMoveRows * kChunks / kMoveThreads;
+    static_assert(kMoveRows <= kMoveThreads, "a thread a row");
+    __shared__ uint32_t src[kMoveRows], dst[kMoveRows];
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
-    const uint32_t lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes, items = n_heads * stretches;
-    auto rows_of = [&](uint32_t item) -> uint32_t {  // rows of the item's sequence that are kept, 0 behind the last item
-        if (item >= items) return 0u;
-        const uint32_t len = a.len[item / stretches / a.kv_heads];
-        return len > a.cap ? 0u : min(len, a.keep);
-    };
-    auto numbers = [&](uint32_t item, uint32_t n, uint32_t (&j)[kMoveEach]) {
-#pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) {
-            const uint32_t i = item % stretches * kRows + x * kPass + r;
-            j[x] = i < n ? a.kept[(size_t)(item / stretches) * a.keep + i] : kNoRow;
-        }
-    };
-    auto places = [&](uint32_t item, const uint32_t (&j)[kMoveEach], uint32_t (&src)[kMoveEach], uint32_t (&dst)[kMoveEach]) {
-        const uint32_t head = item / stretches, h = head % a.kv_heads;
-        const size_t table = (size_t)(head / a.kv_heads) * a.max_pages;
-#pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) {
-            src[x] = dst[x] = kNoRow;
-            if (j[x] == kNoRow) continue;
-            src[x] = pool_row(a, a.table + table, h, j[x]);
-            dst[x] = pool_row(a, a.to + table, h, item % stretches * kRows + x * kPass + r);
-        }
-    };
-    uint32_t item = blockIdx.x, j[kMoveEach], src[kMoveEach], dst[kMoveEach];
-    numbers(item, rows_of(item), j);
-    places(item, j, src, dst);
-    numbers(item + gridDim.x, rows_of(item + gridDim.x), j);
-    uint32_t ahead = rows_of(item + 2u * gridDim.x);
-    for (; item < items; item += gridDim.x) {
-        uint4 k[kMoveEach], v[kMoveEach];
-#pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) {
-            k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
-            if (src[x] == kNoRow) continue;
-            const size_t at = (size_t)src[x] * HD + lane * 8u;
-            k[x] = *(const uint4 *)(a.kp + at);
-            v[x] = *(const uint4 *)(a.vp + at);
-        }
-        uint32_t to[kMoveEach];
-#pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) to[x] = dst[x];
-        places(item + gridDim.x, j, src, dst);
-        numbers(item + 2u * gridDim.x, ahead, j);
-        ahead = rows_of(item + 3u * gridDim.x);
-#pragma unroll
-        for (uint32_t x = 0; x < kMoveEach; ++x) {
-            if (to[x] == kNoRow) continue;
-            const size_t at = (size_t)to[x] * HD + lane * 8u;
-            *(uint4 *)(a.kp + at) = k[x];
-            *(uint4 *)(a.vp + at) = v[x];
-        }
+    const uint32_t s = blockIdx.y / a.kv_heads, h = blockIdx.y % a.kv_heads, len = a.len[s], i0 = blockIdx.x * kMoveRows;
+    if (len > a.cap || i0 >= min(len, a.keep)) return;
+    const uint32_t rows = min(kMoveRows, min(len, a.keep) - i0);
+    if (threadIdx.x < rows) {
+        const uint32_t i = i0 + threadIdx.x, j = a.kept[(size_t)blockIdx.y * a.keep + i];
+        src[threadIdx.x] = pool_row(a, a.table + (size_t)s * a.max_pages, h, j);
+        dst[threadIdx.x] = pool_row(a, a.to + (size_t)s * a.max_pages, h, i);
     }
+    __syncthreads();
+    __half *pool = blockIdx.z ? a.vp : a.kp;
+    uint4 v[kEach];
+    uint32_t to[kEach];
+#pragma unroll
+    for (uint32_t x = 0; x < kEach; ++x) {
+        const uint32_t e = x * kMoveThreads + threadIdx.x, row = e / kChunks, from = row < rows ? src[row] : kNoRow;
+        to[x] = row < rows ? dst[row] : kNoRow;
+        v[x] = from != kNoRow ? *(const uint4 *)(pool + (size_t)from * HD + e % kChunks * 8u) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (uint32_t x = 0; x < kEach; ++x)
+        if (to[x] != kNoRow) *(uint4 *)(pool + (size_t)to[x] * HD + (x * kMoveThreads + threadIdx.x) % kChunks * 8u) = v[x];
 }
 
 // In place: a CTA takes 64 bytes of every row of a head, so that the columns need not wait for one another, and goes up the
@@ -1009,10 +980,8 @@ template <int HD>
 cudaError_t launch_move(tm_cuda_ctx *ctx, const evict_args &a, uint32_t n_seq, bool in_place) {
     if (in_place)
         return tm_launch_pdl(ctx, kv_evict_shift_kernel<HD>, dim3(2 * (HD / 32), n_seq * a.kv_heads), dim3(kMoveThreads), 0, a);
-    const uint32_t rows = kMoveThreads / (HD / 8) * kMoveEach, stretches = (a.keep + rows - 1) / rows, heads = n_seq * a.kv_heads;
-    const uint32_t places = 4u * (uint32_t)ctx->sm_count;
-    const uint32_t ctas = (uint64_t)heads * stretches < places ? heads * stretches : places;
-    return tm_launch_pdl(ctx, kv_evict_move_kernel<HD>, dim3(ctas), dim3(kMoveThreads), 0, a, heads, stretches);
+    return tm_launch_pdl(ctx, kv_evict_move_kernel<HD>, dim3((a.keep + kRowsMoved<HD> - 1) / kRowsMoved<HD>, n_seq * a.kv_heads, 2),
+                         dim3(kMoveThreads), 0, a);
 }
 
 template <int HD>
