@@ -763,13 +763,15 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
                                             uint32_t (&warps)[32], uint32_t (&found)[3]) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
-    const uint32_t strip = (len + kEvictThreads - 1u) / kEvictThreads, j0 = tid * strip;
+    // (Held strips are 4 or 8 rows, whose weights begin on 16 bytes and end within the sequence's: a page has 16 rows or more.)
+    const uint32_t strip = !HELD ? (len + kEvictThreads - 1u) / kEvictThreads : len <= 4u * kEvictThreads ? 4u : 8u, j0 = tid * strip;
     float held[HELD ? kHeld : 1];
     if (HELD) {
 #pragma unroll
-        for (uint32_t e = 0; e < kHeld; ++e) held[HELD ? e : 0] = e < strip && j0 + e < len ? w[j0 + e] : 0.0f;
+        for (uint32_t e = 0; e < kHeld; e += 4)
+            if (e < strip && j0 + e < len) *(float4 *)&held[HELD ? e : 0] = *(const float4 *)(w + j0 + e);
     }
-    // f(row, weight) for the strip's rows
+    // f(row, weight) for the strip's rows; a row of `len` or more has no weight
     auto rows = [&](auto f) {
         if (HELD) {
 #pragma unroll
@@ -820,27 +822,30 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
             __syncthreads();
         }
     }
-    // The rows that stay: keys above the border, and the first `left` at it.
-    uint32_t equal = 0u, total;
-    auto middle = [&](uint32_t j) { return j >= lo && j < hi; };
-    if (want > 0u) rows([&](uint32_t j, float v) { equal += middle(j) && (weight_key(v) & mask) == prefix ? 1u : 0u; });
-    const uint32_t eq = block_scan(equal, warps, total);
-    uint32_t e = eq;
-    auto stays = [&](uint32_t j, float v) {
-        if (j >= len) return false;
-        if (!middle(j)) return true;
-        if (want == 0u) return false;
-        const uint32_t key = weight_key(v) & mask;
-        return key > prefix || (key == prefix && e++ < left);
-    };
-    uint32_t mine = 0u;
-    rows([&](uint32_t j, float v) { mine += stays(j, v) ? 1u : 0u; });
-    uint32_t at = block_scan(mine, warps, total);  // (behind its barriers all weights that are held have been read)
-    e = eq;
+    // The rows that stay: those outside lo .. hi and with keys above the border, and the first `left` at it.
+    auto above = [&](uint32_t j, float v) { return j < len && (j < lo || j >= hi || (want > 0u && (weight_key(v) & mask) > prefix)); };
+    auto equal = [&](uint32_t j, float v) { return j >= lo && j < hi && want > 0u && (weight_key(v) & mask) == prefix; };
+    uint32_t n_above = 0u, n_equal = 0u, total;
     rows([&](uint32_t j, float v) {
-        if (!stays(j, v)) return;
-        if (HELD) w_out[at] = v;
-        kept[at++] = j;
+        n_above += above(j, v) ? 1u : 0u;
+        n_equal += equal(j, v) ? 1u : 0u;
+    });
+    if (HELD) {  // both counts in one sum (behind its barriers all weights have been read)
+        const uint32_t both = block_scan(n_above << 16 | n_equal, warps, total);
+        n_above = both >> 16;
+        n_equal = both & 0xffffu;
+    } else {
+        n_above = block_scan(n_above, warps, total);
+        n_equal = block_scan(n_equal, warps, total);
+    }
+    uint32_t at = n_above + min(n_equal, left);
+    rows([&](uint32_t j, float v) {
+        const bool tie = equal(j, v);
+        if (above(j, v) || (tie && n_equal < left)) {
+            if (HELD) w_out[at] = v;
+            kept[at++] = j;
+        }
+        n_equal += tie ? 1u : 0u;
     });
 }
 
