@@ -60,6 +60,10 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // it.  Three launches: the vectors (queries and new rows: norm, rotation, f16), the rows, and the join of what the warps
 // have found.  The second starts beside the first and waits for it when it has its rows on their way.
 //
+// What it measured (8 KV heads of 128): the rows of one sequence of 131071 (537 MB) 86 us, 6.2 TB/s, of 32 up to 4095 (343 MB
+// with the scores) 60 us, 5.7 TB/s; around them 3 us until the first rows arrive and 3 to 7 us of the join.  (Slices whose
+// last eighth went to whichever warp was free measured the same: what ends late waits for the memory, not for work.)
+//
 // A warp takes 16 rows of each tile through its own ring of cp.async stages and keeps its own running (max, sum, output):
 // the warps of a CTA never meet (with the pieces of a pair combined in the CTA, barriers and the next pair's queries took
 // 7000 cycles a pair, as long as 250 rows).  The ring runs on across pairs.  Both products are mma.m16n8k16 with the cached
@@ -128,28 +132,48 @@ struct line {
         return t < longer ? t / (each + 1u) : extra + (t - longer) / each;
     }
 };
+// The sequences' lengths.  The second and third launch read them (and pages, cached rows, earlier weights) before their waits:
+// all that has been complete since before the first let them start.  Until the wait it is read from L2, past whatever an SM
+// has kept; the first 32 stay in the lanes of each warp.
+struct lengths {
+    uint32_t held;
+    __device__ __forceinline__ lengths(const paged_args &a) {
+        const uint32_t lane = threadIdx.x & 31u;
+        held = lane < a.n_seq ? __ldcg(a.len + lane) : kSeqNone;
+    }
+    __device__ __forceinline__ uint32_t lane_of(const paged_args &a, uint32_t s0) const {  // of sequence s0 + lane
+        const uint32_t s = s0 + (threadIdx.x & 31u);
+        return s0 == 0u ? held : s < a.n_seq ? __ldcg(a.len + s) : kSeqNone;
+    }
+    __device__ __forceinline__ uint32_t of(const paged_args &a, uint32_t s) const {  // the same sequence for all lanes
+        return s < 32u ? __shfl_sync(0xffffffffu, held, s) : __ldcg(a.len + s);
+    }
+};
 // Tiles of one head's pairs of the sequences below `upto` (whole warps call it).
-__device__ __forceinline__ uint32_t tiles_before(uint32_t upto, const paged_args &a) {
+__device__ __forceinline__ uint32_t tiles_before(const lengths &lens, uint32_t upto, const paged_args &a) {
     uint32_t n = 0;
-    for (uint32_t s = threadIdx.x & 31u; s < upto; s += 32u) n += pair_tiles(a.len[s], a);
+    for (uint32_t s0 = 0; s0 < upto; s0 += 32u) {
+        const uint32_t tiles = pair_tiles(lens.lane_of(a, s0), a);
+        n += s0 + (threadIdx.x & 31u) < upto ? tiles : 0u;
+    }
     return __reduce_add_sync(0xffffffffu, n);
 }
 
 // A tile of the line.
 struct cursor {
     uint32_t s, pair, t, nt, len, start;
-    __device__ __forceinline__ void enter(const paged_args &a) {
-        len = a.len[s];
+    __device__ __forceinline__ void enter(const paged_args &a, uint32_t rows) {
+        len = rows;
         nt = pair_tiles(len, a);
         start = first_row(len, a.window);
     }
     // To the next pair; behind the last one of all it stays at a sequence that is none.
-    __device__ __forceinline__ void next_pair(const paged_args &a) {
+    __device__ __forceinline__ void next_pair(const lengths &lens, const paged_args &a) {
         t = 0;
         if (++pair < a.kv_heads * a.blocks) return;
         pair = 0;
         for (++s; s < a.n_seq; ++s) {
-            enter(a);
+            enter(a, lens.of(a, s));
             if (nt != 0u) break;
         }
     }
@@ -255,7 +279,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
 
     // ---- this CTA's run of tiles ----
     const uint32_t pairs = a.kv_heads * a.blocks;
-    const line all(tiles_before(a.n_seq, a) * pairs, a);
+    const lengths lens(a);
+    const line all(tiles_before(lens, a.n_seq, a) * pairs, a);
     if (blockIdx.x >= all.ctas) {
         tmdev::pdl_wait();
         return;
@@ -267,7 +292,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
         uint32_t before = 0;  // tiles of the sequences before the one that tile u0 belongs to
         at.s = 0;
         for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32u) {
-            const uint32_t n = s0 + lane < a.n_seq ? pair_tiles(a.len[s0 + lane], a) * pairs : 0u;
+            const uint32_t n = pair_tiles(lens.lane_of(a, s0), a) * pairs;
             uint32_t incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -283,7 +308,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
         }
-        at.enter(a);
+        at.enter(a, lens.of(a, at.s));
         at.pair = (u0 - before) / at.nt;
         at.t = (u0 - before) % at.nt;
     }
@@ -299,9 +324,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
     };
     auto block_of = [&](const cursor &c) { return (c.start / kTile + c.t) * kAttnWarps + warp; };
     auto in_sight = [](const cursor &c, uint32_t blk) { return blk * kBlock <= c.len && blk * kBlock + (kBlock - 1u) >= c.start; };
-    auto ask = [&] {
-        const uint32_t blk = block_of(ahead);
-        ahead_id = in_sight(ahead, blk) ? a.table[(size_t)ahead.s * a.max_pages + (blk * kBlock >> a.page_log)] : 0u;
+    auto ask = [&](bool first) {
+        const uint32_t blk = block_of(ahead), *page = a.table + (size_t)ahead.s * a.max_pages + (blk * kBlock >> a.page_log);
+        ahead_id = !in_sight(ahead, blk) ? 0u : first ? __ldcg(page) : *page;
     };
     auto load = [&](bool first) {
         if (coming != 0u) {
@@ -322,14 +347,14 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
                 }
             }
             if (--coming != 0u) {
-                if (++ahead.t >= ahead.nt) ahead.next_pair(a);
-                ask();
+                if (++ahead.t >= ahead.nt) ahead.next_pair(lens, a);
+                ask(first);
             }
         }
         fill = fill + 1u == STAGES ? 0u : fill + 1u;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    ask();
+    ask(true);
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) load(true);
     wait();
@@ -448,7 +473,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             }
         }
         left -= tn;
-        if (left != 0u) at.next_pair(a);
+        if (left != 0u) at.next_pair(lens, a);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -464,7 +489,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(c
     __shared__ float sm[32], sl[32], so[kJoinWarps][DIMS];
     tmdev::pdl_trigger();
     const uint32_t s = blockIdx.y, tid = threadIdx.x, warp = tmdev::warp_index(), lane = tid & 31u;
-    const uint32_t len = a.len[s], nt = pair_tiles(len, a), joining = a.heads * kParts;
+    const lengths lens(a);
+    const uint32_t len = lens.of(a, s), nt = pair_tiles(len, a), joining = a.heads * kParts;
     const bool joins = blockIdx.x < joining;
     const uint32_t head = blockIdx.x / kParts, d0 = blockIdx.x % kParts * DIMS;  // (of one that joins)
     const uint32_t kvh = joins ? head / a.group : (blockIdx.x - joining) % a.kv_heads;
@@ -480,12 +506,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(c
 #pragma unroll
         for (uint32_t r = 0; r < kCountEach; ++r) {
             const uint32_t j = row0 + r * kJoinThreads + tid;
-            w[r] = a.w_in && j < len ? a.w_in[base + j] : 0.0f;  // the new row has drawn nothing before
+            w[r] = a.w_in && j < len ? __ldcg(a.w_in + base + j) : 0.0f;  // the new row has drawn nothing before
         }
     }
     const uint32_t pairs = a.kv_heads * a.blocks;
-    const line all(tiles_before(a.n_seq, a) * pairs, a);
-    const uint32_t before = tiles_before(s, a) * pairs;
+    const line all(tiles_before(lens, a.n_seq, a) * pairs, a);
+    const uint32_t before = tiles_before(lens, s, a) * pairs;
     // The pieces of a head: `n` of them, 4 a CTA; CTA i0 has begun the pair, the others carry on.
     struct pieces {
         uint32_t n;
@@ -658,7 +684,8 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
 // ---- copies between dense planes and pages ---------------------------------------------------------
 //
 // Moves 4 head_dim bytes a row and KV head each way and computes nothing: 16 bytes a thread and load, all loads of a
-// thread before its first store.  A CTA takes up to 64 rows of one run, one head, keys or values.
+// thread before its first store.  A CTA takes up to 64 rows of one run, one head, keys or values.  Bound by the memory:
+// 670 MB (32 sequences of up to 4096 rows, 8 heads of 128) 89 us, 7.5 TB/s of reads and writes together.
 constexpr uint32_t kCopyRows = 64, kCopyThreads = 256;
 struct copy_runs {
     uint32_t n;
@@ -714,8 +741,9 @@ __global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const copy_
 // Per (sequence, KV head): the first `first` rows, the last `recent` rows, and of those between the ones with the largest
 // weights, `keep` in all, in their order.  One CTA finds the smallest weight that stays by counting passes over 11, 11 and
 // 10 bits of the weights' order-preserving integers, then lists the rows; a second launch moves them.  Each thread looks
-// after a strip of consecutive rows, whose weights it holds in registers up to 4096 rows.  What bounds it: the rows' bytes,
-// 8 head_dim each.
+// after a strip of consecutive rows, whose weights it holds in registers up to 4096 rows, so that a pass is counting alone
+// (256 heads of up to 4096 rows: 14 us, a third of it the first pass, whose digits are few; weights read again for every
+// pass by 1024 threads 19).  What bounds the whole: the rows' bytes, 8 head_dim each.
 constexpr uint32_t kEvictThreads = 512;
 
 struct evict_args {
@@ -905,7 +933,8 @@ __device__ __forceinline__ uint32_t pool_row(const evict_args &a, const uint32_t
 
 // Into other pages: a CTA takes 16 KB of a head's rows, keys or values.  A row's place is behind two loads that depend on one
 // another (its number, its page): a thread a row looks them up, then all copy as in kv_pages_copy_kernel.  Many small CTAs
-// hide that better than few that look ahead (32 sequences of 4096 rows, half of them kept: X us instead of 93).
+// hide that better than few that look two stretches ahead (32 sequences of 4096 rows cut to 2048, 493 MB: 76 us, 6.5 TB/s;
+// 86 us; 8 KB a CTA 84).
 template <int HD>
 constexpr uint32_t kRowsMoved = 8192u / HD;
 template <int HD>
@@ -1203,8 +1232,6 @@ int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_bu
     if (keep == 0 || keep > cap || (uint64_t)first + recent > keep)
         return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: keep %u of at most %zu rows, the first %u and the last %u among them",
                        keep, cap, first, recent);
-    if ((uint64_t)n_seq * kv_heads * keep > 0x7fffffffu)
-        return tm_fail(err, err_cap, TM_CUDA_ERR_BOUNDS, "eviction: %u rows of %u sequences of %u KV heads", keep, n_seq, kv_heads);
     const size_t nw = (size_t)n_seq * kv_heads * cap * 4, nk = (size_t)n_seq * kv_heads * keep * 4;
     const size_t ntable = (size_t)n_seq * max_pages * 4, nlen = (size_t)n_seq * 4;
     TM_CHECK_BUF(k_pages, pool_bytes(shape), "K pages");
