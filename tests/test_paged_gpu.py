@@ -601,6 +601,14 @@ EVICT = [
     ([5000], 2, 64, 128, 2100, 4, 64),
     ([9000, 4096, 4097, 3000], 1, 32, 256, 2500, 1, 70),  # on both sides of what registers hold
     ([3000], 1, 32, 64, 1500, 0, 0),
+    # few heads, long sequences: a cluster of 8, 4 or 2 CTAs a head, weights in its registers or read again
+    ([20000, 0, 2049, 900], 2, 32, 256, 8000, 5, 33),
+    ([32768], 1, 32, 256, 5000, 0, 0),
+    ([40000, 32769, 100, 4100], 1, 32, 256, 6000, 0, 100),
+    ([33000], 1, 32, 256, 700, 300, 400),
+    ([16384, 16390], 20, 32, 256, 300, 3, 7),
+    ([9000, 8192, 4097], 25, 32, 128, 257, 3, 7),
+    ([4200], 150, 32, 256, 30, 1, 2),  # more heads than that: one CTA each
 ]
 
 

@@ -6,8 +6,9 @@
 // CTA reads the row's whole log and bias map (a few kilobytes that the row's CTAs share in L2) and counts the tokens of its
 // own stretch with integer atomics, whose order does not matter, while its logits are on their way into registers.  The
 // arithmetic is done once for each named token; all other logits pass from registers to memory
-// under the mask (words tested for every logit: 32 rows of 151936 34 us instead of 16.7; the log read once by a cluster of
-// CTAs that send each other its entries: 19.4).  Each step is rounded to f32 by itself, so a choice does not hang on how an
+// under the mask (words tested for every logit: 32 rows of 151936 34 us instead of 17.3; the log read once by a cluster of
+// CTAs that send each other its entries: 19.4 instead of 16.7 then; one word a quad worked out before from mask and bits, so
+// that each has fewer instructions but all wait for it: 17.1, 25.7 instead of 25.1 for 48 rows of 262144).  Each step is rounded to f32 by itself, so a choice does not hang on how an
 // expression was contracted.
 #include "tm_cuda_internal.cuh"
 #include "tm_cuda_device.cuh"
@@ -158,12 +159,26 @@ __global__ void __launch_bounds__(kThreads, EACH == 8 ? 4 : 5) logits_adjust_ker
     }
     uint32_t best_at = kNone;
     if (a.partial && mine != 0u) {
-        const bool found = best > -INFINITY;  // else the first that is -infinity and no NaN, whatever its quad
+        if (best > -INFINITY) {
+            float q[4];
+            uint32_t of = 0u;
 #pragma unroll
-        for (int e = EACH - 1; e >= 0; --e)
+            for (int e = 0; e < EACH; ++e) {
+                if (best_quad != e) continue;
+                of = mine >> (4 * e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = v[e][k];
+            }
 #pragma unroll
             for (int k = 3; k >= 0; --k)
-                if (v[e][k] == best && (mine >> (4 * e + k) & 1u) != 0u && (!found || best_quad == e)) best_at = c0 + (e * kThreads + tid) * 4u + k;
+                if (q[k] == best && (of >> k & 1u) != 0u) best_at = c0 + (best_quad * kThreads + tid) * 4u + k;
+        } else {  // the first that is -infinity and no NaN
+#pragma unroll
+            for (int e = EACH - 1; e >= 0; --e)
+#pragma unroll
+                for (int k = 3; k >= 0; --k)
+                    if (v[e][k] == best && (mine >> (4 * e + k) & 1u) != 0u) best_at = c0 + (e * kThreads + tid) * 4u + k;
+        }
     }
     // ---- the others ----
     const float repetition = a.penalties ? a.penalties[r * 3] : 1.0f, presence = a.penalties ? a.penalties[r * 3 + 1] : 0.0f;
@@ -296,12 +311,13 @@ int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_c
     a.bias_cap = bias_cap;
     a.mask_words = words;
     a.log_cap = log_cap;
-    // Stretches of 1024 logits keep every SM busy with one row (151936 logits, a log of 600: 4.2 us); with many rows longer
-    // ones, because every CTA reads the row's log (32 rows of 151936, logs up to 4000, a mask and a bias map: 2048 logits
-    // 20.9 us, 4096 16.8, 8192 16.7; 48 of 262144, logs up to 1200: 36.6, 29.6, 27.4, floor 15.7).
-    const uint32_t most = 4u * (uint32_t)ctx->sm_count;
+    // Short stretches keep every SM busy with few rows (one of 151936 logits, a log of 600, 1024 logits: 4.3 us), as long as all
+    // find a place at once (8 rows, 2048 logits 8.1 us, 4096 9.1; 16 rows, 4096 11.0, 8192 13.4); with many rows long ones,
+    // because every CTA reads the row's log (32 rows, logs up to 4000, a mask and a bias map: 4096 logits 18.2, 8192 17.3; 48 of
+    // 262144, logs up to 1200: 29, 25.1, floor 15.7).
+    const uint32_t sms = (uint32_t)ctx->sm_count;
     uint32_t each = 1;
-    while (each < 8u && ((n + each * 1024u - 1) / (each * 1024u) > kMostChunks || (uint64_t)n_rows * ((n + each * 1024u - 1) / (each * 1024u)) > most))
+    while (each < 8u && ((n + each * 1024u - 1) / (each * 1024u) > kMostChunks || (uint64_t)n_rows * ((n + each * 1024u - 1) / (each * 1024u)) > 5u * sms))
         each *= 2;
     const uint32_t chunks = (n + each * 1024u - 1) / (each * 1024u);
     TM_OP_BEGIN("logits_adjust_rows");

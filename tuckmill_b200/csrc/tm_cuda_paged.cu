@@ -661,7 +661,7 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
         if (device >= 0 && device < 64) attr_done[device].store(true, std::memory_order_release);
     }
     // At most: tiles of a pair, pairs, and with these the CTAs.
-    const uint32_t whole = (a.cap + kTile - 1) / kTile, seen = a.window ? (a.window + kTile - 2) / kTile + 1u : whole;
+    const uint32_t whole = (a.cap + kTile - 1) / kTile, seen = a.window && a.window < a.cap ? (a.window + kTile - 2) / kTile + 1u : whole;
     const uint32_t tiles = seen < whole ? seen : whole, pairs = a.n_seq * a.kv_heads * a.blocks;
     const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), most_ctas(HD));
     a.ctas = (uint32_t)min((uint64_t)tiles * pairs, (uint64_t)places);
@@ -739,11 +739,12 @@ __global__ void __launch_bounds__(kCopyThreads) kv_pages_copy_kernel(const copy_
 // ---- eviction --------------------------------------------------------------------------------------
 //
 // Per (sequence, KV head): the first `first` rows, the last `recent` rows, and of those between the ones with the largest
-// weights, `keep` in all, in their order.  One CTA finds the smallest weight that stays by counting passes over 11, 11 and
-// 10 bits of the weights' order-preserving integers, then lists the rows; a second launch moves them.  Each thread looks
-// after a strip of consecutive rows, whose weights it holds in registers up to 4096 rows, so that a pass is counting alone
-// (256 heads of up to 4096 rows: 14 us, a third of it the first pass, whose digits are few; weights read again for every
-// pass by 1024 threads 19).  What bounds the whole: the rows' bytes, 8 head_dim each.
+// weights, `keep` in all, in their order.  One CTA, or a cluster, finds the smallest weight that stays by counting passes over 11, 11
+// and 10 bits of the weights' order-preserving integers, then lists the rows; a second launch moves them.  Up to 4096 rows the
+// weights stay in registers, so that a pass is counting alone: 256 heads of up to 4096 rows 13 us.  (Every count adds the
+// constant one, which shared memory takes for a whole warp at once whatever the digits: with zeros counted by ballot, so that
+// few lanes add to their bin, 14, and with all equal digits of a warp found first 33.)  What bounds the whole: the rows'
+// bytes, 8 head_dim each.
 constexpr uint32_t kEvictThreads = 512;
 
 struct evict_args {
@@ -785,138 +786,212 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *warps, uint
     return __shfl_sync(0xffffffffu, sum - w, warp) + incl - v;
 }
 
-constexpr uint32_t kHeld = 8;  // weights of a strip in registers
-template <bool HELD>
-__device__ __forceinline__ void select_rows(const evict_args &a, const float *w, float *w_out, uint32_t *kept, uint32_t len, uint32_t (&hist)[2048],
-                                            uint32_t (&warps)[32], uint32_t (&found)[3]) {
-    const uint32_t tid = threadIdx.x, lane = tid & 31u;
+constexpr uint32_t kHeld = 8, kStretch = kHeld * kEvictThreads;  // weights of a thread in registers, of a CTA
+struct select_smem {
+    uint32_t hist[2][2048];
+    uint32_t warps[32], found[3];
+    uint32_t above, equal;  // rows of this CTA that stay, and at the border
+};
+template <uint32_t CTAS>
+__device__ __forceinline__ void sync_all() {
+    if (CTAS == 1u) __syncthreads();
+    else tmdev::cluster_sync();
+}
+__device__ __forceinline__ uint32_t ld_rank(const uint32_t *p, uint32_t rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(tmdev::map_rank(smem_addr(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 ld_rank4(const uint32_t *p, uint32_t rank) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(tmdev::map_rank(smem_addr(p), rank)) : "memory");
+    return v;
+}
+
+// Of a head's rows this CTA (`rank` of CTAS, a cluster) looks after r0 .. r1.  HELD: their weights stay in registers (at most a
+// stretch of them); else they are read again for every pass, a stretch ahead.
+template <bool HELD, uint32_t CTAS>
+__device__ __forceinline__ void select_rows(const evict_args &a, const float *w, float *w_out, uint32_t *kept, uint32_t len, uint32_t rank,
+                                            select_smem &sm) {
+    const uint32_t tid = threadIdx.x;
+    const uint32_t per = (len + 16u * CTAS - 1u) / (16u * CTAS) * 16u, r0 = min(len, rank * per), r1 = min(len, r0 + per);
     const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
-    // (Held strips are 4 or 8 rows, whose weights begin on 16 bytes and end within the sequence's: a page has 16 rows or more.)
-    const uint32_t strip = !HELD ? (len + kEvictThreads - 1u) / kEvictThreads : len <= 4u * kEvictThreads ? 4u : 8u, j0 = tid * strip;
-    float held[HELD ? kHeld : 1];
-    if (HELD) {
+    // (Strips are 4 or 8 rows, whose weights begin on 16 bytes and end within the sequence's: a page has 16 rows or more.)
+    const uint32_t strip = HELD && per <= 4u * kEvictThreads ? 4u : 8u, j0 = r0 + tid * strip;
+    float held[kHeld];
+    auto fetch = [&](float(&v)[kHeld], uint32_t at, uint32_t step) {  // rows at .. at + 3 and, of strips of 8, at + step .. at + step + 3
 #pragma unroll
-        for (uint32_t e = 0; e < kHeld; e += 4)
-            if (e < strip && j0 + e < len) *(float4 *)&held[HELD ? e : 0] = *(const float4 *)(w + j0 + e);
-    }
-    // f(row, weight) for the strip's rows; a row of `len` or more has no weight
-    auto rows = [&](auto f) {
-        if (HELD) {
-#pragma unroll
-            for (uint32_t e = 0; e < kHeld; ++e)
-                if (e < strip) f(j0 + e, held[HELD ? e : 0]);
-        } else {
-            for (uint32_t e = 0; e < strip; ++e) f(j0 + e, j0 + e < len ? w[j0 + e] : 0.0f);
-        }
+        for (uint32_t e = 0; e < 2; ++e)
+            if (4u * e < strip && at + e * step < r1) *(float4 *)&v[4 * e] = *(const float4 *)(w + at + e * step);
     };
+    if (HELD) fetch(held, j0, 4u);
     // The want-th largest key between lo and hi, digit by digit: `prefix` its bits so far (those of `mask`), `left` how many
     // are still wanted among the keys that begin with them.
     uint32_t prefix = 0u, mask = 0u, left = want;
+    auto equal = [&](uint32_t j, float v) {  // (a row behind r1 has no weight)
+        return j >= lo && j < hi && j < r1 && want > 0u && (weight_key(v) & mask) == prefix;
+    };
+    auto above = [&](uint32_t j, float v) { return j < r1 && (j < lo || j >= hi || (want > 0u && (weight_key(v) & mask) > prefix)); };
+    auto in_any_order = [&](auto f) {  // f(row, weight), as it loads best
+        fetch(held, r0 + 4u * tid, kStretch / 2);
+#pragma unroll 1
+        for (uint32_t s0 = r0; s0 < r1; s0 += kStretch) {
+            const uint32_t at = s0 + 4u * tid;
+            float next[kHeld];
+            fetch(next, at + kStretch, kStretch / 2);
+#pragma unroll
+            for (uint32_t e = 0; e < kHeld; ++e) f(at + e / 4u * (kStretch / 2) + e % 4u, held[e]);
+#pragma unroll
+            for (uint32_t e = 0; e < kHeld; ++e) held[e] = next[e];
+        }
+    };
     if (want > 0u) {
         const uint32_t shift[3] = {21u, 10u, 0u}, width[3] = {11u, 11u, 10u};
 #pragma unroll 1
-        for (int p = 0; p < 3; ++p) {
+        for (uint32_t p = 0; p < 3u; ++p) {
+            uint32_t *hist = sm.hist[p & 1u];  // (the other one may still be read by the other CTAs)
             *(uint4 *)(hist + 4u * tid) = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
             const uint32_t digits = (1u << width[p]) - 1u;
-            rows([&](uint32_t j, float v) {
-                const uint32_t key = weight_key(v);
-                const bool mine = j >= lo && j < hi && (key & mask) == prefix;
-                // rows that nothing has looked at tie: a warp counts its zeros at once
-                const uint32_t zeros = __ballot_sync(0xffffffffu, mine && key == 0x80000000u);
-                if (mine && (key != 0x80000000u || lane == (uint32_t)__ffs(zeros) - 1u))
-                    atomicAdd(&hist[(key >> shift[p]) & digits], key != 0x80000000u ? 1u : (uint32_t)__popc(zeros));
-            });
-            __syncthreads();
+            auto count = [&](uint32_t j, float v) {
+                if (equal(j, v)) atomicAdd(&hist[(weight_key(v) >> shift[p]) & digits], 1u);
+            };
+            if (HELD) {
+#pragma unroll
+                for (uint32_t e = 0; e < kHeld; ++e)
+                    if (e < strip) count(j0 + e, held[e]);
+            } else {
+                in_any_order(count);
+            }
+            sync_all<CTAS>();
             // Thread i: four bins from 2047 - 4i down, so that a prefix sum counts from the top.
             const uint32_t b = 2044u - 4u * tid;
-            const uint4 c = *(const uint4 *)(hist + b);
-            uint32_t total, above = block_scan(c.x + c.y + c.z + c.w, warps, total);
+            uint4 c = *(const uint4 *)(hist + b);
+#pragma unroll
+            for (uint32_t i = 1; i < CTAS; ++i) {
+                const uint4 o = ld_rank4(hist + b, (rank + i) % CTAS);
+                c = make_uint4(c.x + o.x, c.y + o.y, c.z + o.z, c.w + o.w);
+            }
+            uint32_t total, before = block_scan(c.x + c.y + c.z + c.w, sm.warps, total);
             const uint32_t of[4] = {c.w, c.z, c.y, c.x};
 #pragma unroll
             for (uint32_t x = 0; x < 4u; ++x) {
-                if (above < left && above + of[x] >= left) {
-                    found[0] = b + 3u - x;
-                    found[1] = left - above;
-                    found[2] = of[x];
+                if (before < left && before + of[x] >= left) {
+                    sm.found[0] = b + 3u - x;
+                    sm.found[1] = left - before;
+                    sm.found[2] = of[x];
                 }
-                above += of[x];
+                before += of[x];
             }
             __syncthreads();
-            prefix |= found[0] << shift[p];
+            prefix |= sm.found[0] << shift[p];
             mask |= digits << shift[p];
-            left = found[1];
-            if (found[2] == left) break;  // all that begin with these bits stay
-            __syncthreads();
+            left = sm.found[1];
+            if (sm.found[2] == left) break;  // all that begin with these bits stay
         }
     }
-    // The rows that stay: those outside lo .. hi and with keys above the border, and the first `left` at it.
-    auto above = [&](uint32_t j, float v) { return j < len && (j < lo || j >= hi || (want > 0u && (weight_key(v) & mask) > prefix)); };
-    auto equal = [&](uint32_t j, float v) { return j >= lo && j < hi && want > 0u && (weight_key(v) & mask) == prefix; };
-    uint32_t n_above = 0u, n_equal = 0u, total;
-    rows([&](uint32_t j, float v) {
-        n_above += above(j, v) ? 1u : 0u;
-        n_equal += equal(j, v) ? 1u : 0u;
-    });
-    if (HELD) {  // both counts in one sum (behind its barriers all weights have been read)
-        const uint32_t both = block_scan(n_above << 16 | n_equal, warps, total);
-        n_above = both >> 16;
-        n_equal = both & 0xffffu;
-    } else {
-        n_above = block_scan(n_above, warps, total);
-        n_equal = block_scan(n_equal, warps, total);
-    }
-    uint32_t at = n_above + min(n_equal, left);
-    rows([&](uint32_t j, float v) {
-        const bool tie = equal(j, v);
-        if (above(j, v) || (tie && n_equal < left)) {
-            if (HELD) w_out[at] = v;
-            kept[at++] = j;
+    // The rows that stay: those outside lo .. hi and with keys above the border, and the first `left` at it.  Counted and listed
+    // stretch by stretch, in order; `stay` and `ties` are those before the stretch.
+    uint32_t stay = 0u, ties = 0u, total;
+    auto counts = [&](uint32_t s0) {  // of this thread's strip: rows above in the upper half, at the border in the lower
+        uint32_t both = 0u;
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e)
+            if (e < strip) both += (above(s0 + e, held[e]) ? 1u << 16 : 0u) + (equal(s0 + e, held[e]) ? 1u : 0u);
+        return both;
+    };
+    uint32_t both = 0u;
+    if (CTAS > 1u) {  // what the CTAs before this one have
+        if (HELD) {
+            both = block_scan(counts(j0), sm.warps, total);
+            if (tid == 0) {
+                sm.above = total >> 16;
+                sm.equal = total & 0xffffu;
+            }
+        } else {
+            uint32_t n_above = 0u, n_equal = 0u;
+            in_any_order([&](uint32_t j, float v) {
+                n_above += above(j, v) ? 1u : 0u;
+                n_equal += equal(j, v) ? 1u : 0u;
+            });
+            block_scan(n_above, sm.warps, total);
+            if (tid == 0) sm.above = total;
+            block_scan(n_equal, sm.warps, total);
+            if (tid == 0) sm.equal = total;
         }
-        n_equal += tie ? 1u : 0u;
-    });
+        tmdev::cluster_sync();  // (all that is HELD has been read)
+        for (uint32_t i = 0; i < rank; ++i) {
+            stay += ld_rank(&sm.above, i);
+            ties += ld_rank(&sm.equal, i);
+        }
+        if (HELD) tmdev::cluster_arrive();  // nothing of another CTA's is read from here on
+    }
+#pragma unroll 1
+    for (uint32_t s0 = 0; s0 < r1 - r0; s0 += kStretch) {
+        if (!HELD) fetch(held, s0 + j0, 4u);
+        if (!HELD || CTAS == 1u) both = block_scan(counts(s0 + j0), sm.warps, total);  // behind it the stretch's weights are read
+        uint32_t n_equal = ties + (both & 0xffffu), at = stay + (both >> 16) + min(n_equal, left);
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e) {
+            const uint32_t j = s0 + j0 + e;
+            if (e >= strip) continue;
+            const bool tie = equal(j, held[e]);
+            if (above(j, held[e]) || (tie && n_equal < left)) {
+                // what stays moves down, if at all: weights_out may be the weights themselves
+                if (HELD || CTAS == 1u) w_out[at] = held[e];
+                kept[at++] = j;
+            }
+            n_equal += tie ? 1u : 0u;
+        }
+        stay += total >> 16;
+        ties += total & 0xffffu;
+    }
+    if (CTAS > 1u && HELD) tmdev::cluster_wait();
+    if (CTAS > 1u && !HELD) {  // the others may still have to read what this CTA would overwrite: the weights follow together
+        tmdev::cluster_sync();
+        for (uint32_t i0 = 0; i0 < a.keep; i0 += CTAS * kEvictThreads) {
+            const uint32_t i = i0 + rank * kEvictThreads + tid;
+            const float v = i < a.keep ? w[kept[i]] : 0.0f;
+            tmdev::cluster_sync();
+            if (i < a.keep) w_out[i] = v;
+            tmdev::cluster_sync();
+        }
+    }
 }
 
+// A head's rows are looked after by one CTA, or where there are few heads and a head may have more than a stretch by a cluster.
+template <uint32_t CTAS>
 __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const evict_args a) {
-    __shared__ __align__(16) uint32_t hist[2048];
-    __shared__ uint32_t warps[32], found[3];
+    __shared__ __align__(16) select_smem sm;
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
-    const uint32_t s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, len = a.len[s];
+    const uint32_t s = blockIdx.y, h = blockIdx.x / CTAS, rank = blockIdx.x % CTAS, tid = threadIdx.x, len = a.len[s];
     if (len == kSeqNone || len > a.cap) {
-        if (h == 0 && tid == 0) {
+        if (h == 0 && rank == 0 && tid == 0) {
             if (len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
             if (a.len_out) a.len_out[s] = len;
         }
         return;
     }
-    if (a.len_out && h == 0 && tid == 0) a.len_out[s] = min(len, a.keep);
+    if (a.len_out && h == 0 && rank == 0 && tid == 0) a.len_out[s] = min(len, a.keep);
     const size_t head = (size_t)s * a.kv_heads + h;
     const float *w = a.w + head * a.cap;
     float *w_out = a.w_out + head * a.cap;
     uint32_t *kept = a.kept + head * a.keep;
-    const uint32_t n = min(len, a.keep);
     if (len <= a.keep) {
-        for (uint32_t i = tid; i < a.keep; i += kEvictThreads) {
+        for (uint32_t i = rank * kEvictThreads + tid; i < a.keep; i += CTAS * kEvictThreads) {
             kept[i] = i < len ? i : TM_CUDA_SEQ_NONE;
             if (i < len && w_out != w) w_out[i] = w[i];
         }
         return;
     }
-    if (len <= kHeld * kEvictThreads) {
-        select_rows<true>(a, w, w_out, kept, len, hist, warps, found);
+    if (len <= kStretch) {  // (the others have nothing to do)
+        if (rank == 0) select_rows<true, 1>(a, w, w_out, kept, len, 0u, sm);
         return;
     }
-    select_rows<false>(a, w, w_out, kept, len, hist, warps, found);
-    __syncthreads();
-    // The weights go with their rows.  A row never moves up, so reading a stretch before it is written is enough in place.
-    for (uint32_t i0 = 0; i0 < n; i0 += kEvictThreads) {
-        const uint32_t i = i0 + tid;
-        const float v = i < n ? w[kept[i]] : 0.0f;
-        __syncthreads();
-        if (i < n) w_out[i] = v;
-        __syncthreads();
-    }
+    if (len <= CTAS * kStretch) select_rows<true, CTAS>(a, w, w_out, kept, len, rank, sm);
+    else select_rows<false, CTAS>(a, w, w_out, kept, len, rank, sm);
 }
 
 // Moves the kept rows.
@@ -1258,7 +1333,16 @@ int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_bu
                           (uint32_t *)kept->dev, (uint32_t *)status->dev, kv_heads, pages, log2_of(page_rows), max_pages,
                           (uint32_t)cap, keep, first, recent};
     TM_OP_BEGIN("kv_pages_evict");
-    TM_CUDA_TRY(tm_launch_pdl(ctx, kv_evict_select_kernel, dim3(kv_heads, n_seq), dim3(kEvictThreads), 0, a));
+    // Clusters where the heads leave SMs idle and a head may have more than a CTA's registers hold (8 KV heads, one sequence of
+    // 16000 rows cut to 8000: 29.1 us, one CTA a head 35.5; of 120000 cut to 4000: 58, 150; eight of 16000 cut to 200: 19.5, 27.3).
+    const uint64_t heads = (uint64_t)n_seq * kv_heads, room = 2u * (uint32_t)ctx->sm_count;
+    TM_CUDA_TRY(cap <= kStretch || 2u * heads > room
+                    ? tm_launch_pdl(ctx, kv_evict_select_kernel<1>, dim3(kv_heads, n_seq), dim3(kEvictThreads), 0, a)
+                : 4u * heads > room
+                    ? tm_launch_cluster_pdl(ctx, 2, kv_evict_select_kernel<2>, dim3(2 * kv_heads, n_seq), dim3(kEvictThreads), 0, a)
+                : 8u * heads > room
+                    ? tm_launch_cluster_pdl(ctx, 4, kv_evict_select_kernel<4>, dim3(4 * kv_heads, n_seq), dim3(kEvictThreads), 0, a)
+                    : tm_launch_cluster_pdl(ctx, 8, kv_evict_select_kernel<8>, dim3(8 * kv_heads, n_seq), dim3(kEvictThreads), 0, a));
     TM_CUDA_TRY(head_dim == 32    ? launch_move<32>(ctx, a, n_seq, in_place)
                 : head_dim == 64  ? launch_move<64>(ctx, a, n_seq, in_place)
                 : head_dim == 128 ? launch_move<128>(ctx, a, n_seq, in_place)

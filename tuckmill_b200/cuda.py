@@ -534,7 +534,7 @@ class CudaContext:
     def kv_pages_copy(self, k_cache, v_cache, k_pages, v_pages, table, status, pages, page_rows, max_pages, kv_heads,
                       head_dim, cap, to_pages, runs):
         """`runs`: (dense sequence, table row, first row, rows) of each run of rows."""
-        flat = [int(u) for r in runs for u in r]
+        flat = [int(u) for seq, at, first, rows in runs for u in (seq, at, first, rows)]
         self._call("kv_pages_copy_f16", k_cache.handle, v_cache.handle, k_pages.handle, v_pages.handle, table.handle,
                    status.handle, pages, page_rows, max_pages, kv_heads, head_dim, cap, int(to_pages), len(runs),
                    (C.c_uint32 * len(flat))(*flat))
