@@ -792,10 +792,10 @@ struct select_smem {
     uint32_t warps[32], found[3];
     uint32_t above, equal;  // rows of this CTA that stay, and at the border
 };
-template <uint32_t CTAS>
+template <bool MANY>
 __device__ __forceinline__ void sync_all() {
-    if (CTAS == 1u) __syncthreads();
-    else tmdev::cluster_sync();
+    if (MANY) tmdev::cluster_sync();
+    else __syncthreads();
 }
 __device__ __forceinline__ uint32_t ld_rank(const uint32_t *p, uint32_t rank) {
     uint32_t v;
@@ -809,13 +809,14 @@ __device__ __forceinline__ uint4 ld_rank4(const uint32_t *p, uint32_t rank) {
     return v;
 }
 
-// Of a head's rows this CTA (`rank` of CTAS, a cluster) looks after r0 .. r1.  HELD: their weights stay in registers (at most a
-// stretch of them); else they are read again for every pass, a stretch ahead.
-template <bool HELD, uint32_t CTAS>
+// Of a head's rows this CTA (`rank` of `ctas` in a cluster; MANY: more than one; a rank behind them has none) looks after r0 .. r1.  HELD: their weights stay
+// in registers (at most a stretch of them); else they are read again for every pass, a stretch ahead.
+constexpr uint32_t kMostCtas = 8;
+template <bool HELD, bool MANY>
 __device__ __forceinline__ void select_rows(const evict_args &a, const float *w, float *w_out, uint32_t *kept, uint32_t len, uint32_t rank,
-                                            select_smem &sm) {
+                                            uint32_t ctas, select_smem &sm) {
     const uint32_t tid = threadIdx.x;
-    const uint32_t per = (len + 16u * CTAS - 1u) / (16u * CTAS) * 16u, r0 = min(len, rank * per), r1 = min(len, r0 + per);
+    const uint32_t per = (len + 16u * ctas - 1u) / (16u * ctas) * 16u, r0 = min(len, rank * per), r1 = min(len, r0 + per);
     const uint32_t lo = a.first, hi = len - a.recent, want = a.keep - a.first - a.recent;
     // (Strips are 4 or 8 rows, whose weights begin on 16 bytes and end within the sequence's: a page has 16 rows or more.)
     const uint32_t strip = HELD && per <= 4u * kEvictThreads ? 4u : 8u, j0 = r0 + tid * strip;
@@ -864,13 +865,15 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
             } else {
                 in_any_order(count);
             }
-            sync_all<CTAS>();
+            sync_all<MANY>();
             // Thread i: four bins from 2047 - 4i down, so that a prefix sum counts from the top.
             const uint32_t b = 2044u - 4u * tid;
             uint4 c = *(const uint4 *)(hist + b);
 #pragma unroll
-            for (uint32_t i = 1; i < CTAS; ++i) {
-                const uint4 o = ld_rank4(hist + b, (rank + i) % CTAS);
+            for (uint32_t i = 1; i < (MANY ? kMostCtas : 1u); ++i) {
+                const uint32_t of = (rank + i) % kMostCtas;
+                if (of >= ctas) continue;
+                const uint4 o = ld_rank4(hist + b, of);
                 c = make_uint4(c.x + o.x, c.y + o.y, c.z + o.z, c.w + o.w);
             }
             uint32_t total, before = block_scan(c.x + c.y + c.z + c.w, sm.warps, total);
@@ -902,7 +905,7 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
         return both;
     };
     uint32_t both = 0u;
-    if (CTAS > 1u) {  // what the CTAs before this one have
+    if (MANY) {  // what the CTAs before this one have
         if (HELD) {
             both = block_scan(counts(j0), sm.warps, total);
             if (tid == 0) {
@@ -921,7 +924,7 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
             if (tid == 0) sm.equal = total;
         }
         tmdev::cluster_sync();  // (all that is HELD has been read)
-        for (uint32_t i = 0; i < rank; ++i) {
+        for (uint32_t i = 0; i < min(rank, ctas); ++i) {
             stay += ld_rank(&sm.above, i);
             ties += ld_rank(&sm.equal, i);
         }
@@ -930,7 +933,7 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
 #pragma unroll 1
     for (uint32_t s0 = 0; s0 < r1 - r0; s0 += kStretch) {
         if (!HELD) fetch(held, s0 + j0, 4u);
-        if (!HELD || CTAS == 1u) both = block_scan(counts(s0 + j0), sm.warps, total);  // behind it the stretch's weights are read
+        if (!HELD || !MANY) both = block_scan(counts(s0 + j0), sm.warps, total);  // behind it the stretch's weights are read
         uint32_t n_equal = ties + (both & 0xffffu), at = stay + (both >> 16) + min(n_equal, left);
 #pragma unroll
         for (uint32_t e = 0; e < kHeld; ++e) {
@@ -939,7 +942,7 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
             const bool tie = equal(j, held[e]);
             if (above(j, held[e]) || (tie && n_equal < left)) {
                 // what stays moves down, if at all: weights_out may be the weights themselves
-                if (HELD || CTAS == 1u) w_out[at] = held[e];
+                if (HELD || !MANY) w_out[at] = held[e];
                 kept[at++] = j;
             }
             n_equal += tie ? 1u : 0u;
@@ -947,10 +950,10 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
         stay += total >> 16;
         ties += total & 0xffffu;
     }
-    if (CTAS > 1u && HELD) tmdev::cluster_wait();
-    if (CTAS > 1u && !HELD) {  // the others may still have to read what this CTA would overwrite: the weights follow together
+    if (MANY && HELD) tmdev::cluster_wait();
+    if (MANY && !HELD) {  // the others may still have to read what this CTA would overwrite: the weights follow together
         tmdev::cluster_sync();
-        for (uint32_t i0 = 0; i0 < a.keep; i0 += CTAS * kEvictThreads) {
+        for (uint32_t i0 = 0; i0 < a.keep; i0 += ctas * kEvictThreads) {
             const uint32_t i = i0 + rank * kEvictThreads + tid;
             const float v = i < a.keep ? w[kept[i]] : 0.0f;
             tmdev::cluster_sync();
@@ -961,12 +964,13 @@ __device__ __forceinline__ void select_rows(const evict_args &a, const float *w,
 }
 
 // A head's rows are looked after by one CTA, or where there are few heads and a head may have more than a stretch by a cluster.
-template <uint32_t CTAS>
+template <bool MANY>
 __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const evict_args a) {
     __shared__ __align__(16) select_smem sm;
     tmdev::pdl_trigger();
     tmdev::pdl_wait();
-    const uint32_t s = blockIdx.y, h = blockIdx.x / CTAS, rank = blockIdx.x % CTAS, tid = threadIdx.x, len = a.len[s];
+    const uint32_t ctas = MANY ? tmdev::cluster_size() : 1u;
+    const uint32_t s = blockIdx.y, h = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, len = a.len[s];
     if (len == kSeqNone || len > a.cap) {
         if (h == 0 && rank == 0 && tid == 0) {
             if (len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
@@ -980,18 +984,23 @@ __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const ev
     float *w_out = a.w_out + head * a.cap;
     uint32_t *kept = a.kept + head * a.keep;
     if (len <= a.keep) {
-        for (uint32_t i = rank * kEvictThreads + tid; i < a.keep; i += CTAS * kEvictThreads) {
+        for (uint32_t i = rank * kEvictThreads + tid; i < a.keep; i += ctas * kEvictThreads) {
             kept[i] = i < len ? i : TM_CUDA_SEQ_NONE;
             if (i < len && w_out != w) w_out[i] = w[i];
         }
         return;
     }
-    if (len <= kStretch) {  // (the others have nothing to do)
-        if (rank == 0) select_rows<true, 1>(a, w, w_out, kept, len, 0u, sm);
+    if (!MANY) {
+        if (len <= kStretch) select_rows<true, false>(a, w, w_out, kept, len, 0u, 1u, sm);
+        else select_rows<false, false>(a, w, w_out, kept, len, 0u, 1u, sm);
         return;
     }
-    if (len <= CTAS * kStretch) select_rows<true, CTAS>(a, w, w_out, kept, len, rank, sm);
-    else select_rows<false, CTAS>(a, w, w_out, kept, len, rank, sm);
+    // As many as it takes to hold the weights; the others have no rows, but take part in the cluster's barriers.
+    const uint32_t need = (len + kStretch - 1u) / kStretch, work = min(ctas, need);
+    if (work == 1u) {
+        if (rank == 0u) select_rows<true, false>(a, w, w_out, kept, len, 0u, 1u, sm);
+    } else if (len <= work * kStretch) select_rows<true, true>(a, w, w_out, kept, len, rank, work, sm);
+    else select_rows<false, true>(a, w, w_out, kept, len, rank, work, sm);
 }
 
 // Moves the kept rows.
@@ -1333,16 +1342,15 @@ int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_bu
                           (uint32_t *)kept->dev, (uint32_t *)status->dev, kv_heads, pages, log2_of(page_rows), max_pages,
                           (uint32_t)cap, keep, first, recent};
     TM_OP_BEGIN("kv_pages_evict");
-    // Clusters where the heads leave SMs idle and a head may have more than a CTA's registers hold (8 KV heads, one sequence of
-    // 16000 rows cut to 8000: 29.1 us, one CTA a head 35.5; of 120000 cut to 4000: 58, 150; eight of 16000 cut to 200: 19.5, 27.3).
+    // Clusters where the heads leave SMs idle and a head may have more than a CTA's registers hold, of as many CTAs as can have
+    // rows (8 KV heads, one sequence of 16000 rows cut to 200, by 4 CTAs a head: 13.3 us, by 8: 17.4, by one 22.8; of 120000 cut to
+    // 4000, by 8: 56, by one 150; eight of 16000 cut to 200, by 4: 19.5, by one 27.3).
     const uint64_t heads = (uint64_t)n_seq * kv_heads, room = 2u * (uint32_t)ctx->sm_count;
-    TM_CUDA_TRY(cap <= kStretch || 2u * heads > room
-                    ? tm_launch_pdl(ctx, kv_evict_select_kernel<1>, dim3(kv_heads, n_seq), dim3(kEvictThreads), 0, a)
-                : 4u * heads > room
-                    ? tm_launch_cluster_pdl(ctx, 2, kv_evict_select_kernel<2>, dim3(2 * kv_heads, n_seq), dim3(kEvictThreads), 0, a)
-                : 8u * heads > room
-                    ? tm_launch_cluster_pdl(ctx, 4, kv_evict_select_kernel<4>, dim3(4 * kv_heads, n_seq), dim3(kEvictThreads), 0, a)
-                    : tm_launch_cluster_pdl(ctx, 8, kv_evict_select_kernel<8>, dim3(8 * kv_heads, n_seq), dim3(kEvictThreads), 0, a));
+    uint32_t ctas = 1;
+    while (ctas < kMostCtas && ctas * kStretch < cap && 2u * ctas * heads <= room) ctas *= 2;
+    const dim3 grid(ctas * kv_heads, n_seq);
+    TM_CUDA_TRY(ctas == 1 ? tm_launch_pdl(ctx, kv_evict_select_kernel<false>, grid, dim3(kEvictThreads), 0, a)
+                          : tm_launch_cluster_pdl(ctx, ctas, kv_evict_select_kernel<true>, grid, dim3(kEvictThreads), 0, a));
     TM_CUDA_TRY(head_dim == 32    ? launch_move<32>(ctx, a, n_seq, in_place)
                 : head_dim == 64  ? launch_move<64>(ctx, a, n_seq, in_place)
                 : head_dim == 128 ? launch_move<128>(ctx, a, n_seq, in_place)
