@@ -5,10 +5,10 @@
 // whose per-token words fit in shared memory, so nothing the size of the vocabulary is kept between calls or cleared: the
 // CTA reads the row's whole log and bias map (a few kilobytes that the row's CTAs share in L2) and counts the tokens of its
 // own stretch with integer atomics, whose order does not matter, while its logits are on their way into registers.  The
-// arithmetic is done once for each named token; all other logits pass from registers to memory
-// under the mask (words tested for every logit: 32 rows of 151936 34 us instead of 17.3; the log read once by a cluster of
-// CTAs that send each other its entries: 19.4 instead of 16.7 then; one word a quad worked out before from mask and bits, so
-// that each has fewer instructions but all wait for it: 17.1, 25.7 instead of 25.1 for 48 rows of 262144).  Each step is rounded to f32 by itself, so a choice does not hang on how an
+// arithmetic is done once for each named token; all other logits pass from registers to memory under the mask (words tested
+// for every logit: 32 rows of 151936 34 us instead of 17.3; the log read once by a cluster of CTAs that send each other its
+// entries: 19.4; mask and bits worked out for a whole word by one lane, fewer instructions, for which all wait: 17.1, and 25.7
+// instead of 25.1 for 48 rows of 262144).  Each step is rounded to f32 by itself, so a choice does not hang on how an
 // expression was contracted.
 #include "tm_cuda_internal.cuh"
 #include "tm_cuda_device.cuh"
