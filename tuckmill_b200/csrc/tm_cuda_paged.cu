@@ -482,9 +482,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
 // of rows (the CTAs behind those).  What needs neither pieces nor scores is done while the rows are still being read, and
 // every warp finds the maximum of all pieces for itself, so that nothing waits for it but the last sums.
 constexpr uint32_t kCountEach = 4;
-template <int HD, int DIMS, uint32_t kJoinWarps>
+template <int HD, int DIMS, uint32_t kJoinWarps, int kBatch>  // kBatch: pieces of a warp on their way at a time
 __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(const paged_args a) {
-    constexpr int EPL = DIMS / 32, kBatch = EPL == 1 ? 10 : 2;
+    constexpr int EPL = DIMS / 32;
     constexpr uint32_t kParts = HD / DIMS, kJoinThreads = 32 * kJoinWarps, kCountRows = kCountEach * kJoinThreads;
     __shared__ float sm[32], sl[32], so[kJoinWarps][DIMS];
     tmdev::pdl_trigger();
@@ -663,22 +663,27 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
     // At most: tiles of a pair, pairs, and with these the CTAs.
     const uint32_t whole = (a.cap + kTile - 1) / kTile, seen = a.window && a.window < a.cap ? (a.window + kTile - 2) / kTile + 1u : whole;
     const uint32_t tiles = seen < whole ? seen : whole, pairs = a.n_seq * a.kv_heads * a.blocks;
-    const uint32_t places = min((uint32_t)(C::kCtas * ctx->sm_count), most_ctas(HD));
-    a.ctas = (uint32_t)min((uint64_t)tiles * pairs, (uint64_t)places);
+    const uint32_t most = min((uint32_t)(C::kCtas * ctx->sm_count), most_ctas(HD));
+    a.ctas = (uint32_t)min((uint64_t)tiles * pairs, (uint64_t)most);
     const uint64_t vectors = (uint64_t)a.n_seq * (a.heads + a.kv_heads);
     cudaError_t e = tm_launch_pdl(ctx, attention_paged_vectors_kernel<HD>, dim3((uint32_t)((vectors + 7) / 8)), dim3(256), 0, a);
     if (e == cudaSuccess) e = tm_launch_pdl(ctx, attention_paged_kernel<HD>, dim3(a.ctas), dim3(kAttnThreads), C::kBytes, a);
     if (e != cudaSuccess) return e;
-    // The join.  Many heads: a CTA of four warps a head (32 sequences of 1000 rows: 22.4 us, with 16 warps 29.8).  Few: their
-    // dims are cut into CTAs of 32 (8 sequences, window 512, one KV head of 256: 8.6, not cut 10.2), and where a pair may lie
-    // in many pieces 16 warps read them (one of 131071 rows: 93.8, with four 98.2; the window's 36 pieces with 16 10.1).
-    const uint32_t pieces = kAttnWarps * min(tiles, a.ctas / pairs + 2u);
-    const bool few = (uint64_t)a.heads * a.n_seq <= 2u * (uint32_t)ctx->sm_count, deep = few && pieces > 64u;
-    const uint32_t rows = kCountEach * 32u * (deep ? 16u : 4u), count = a.w_out ? a.kv_heads * ((a.cap + rows - 1) / rows) : 0u;
-    const dim3 cut(a.heads * (HD / 32) + count, a.n_seq), uncut(a.heads + count, a.n_seq);
-    return deep  ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 16>, cut, dim3(512), 0, a)
-           : few ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 4>, cut, dim3(128), 0, a)
-                 : tm_launch_pdl(ctx, attention_paged_join_kernel<HD, HD, 4>, uncut, dim3(128), 0, a);
+    // The join.  Heads that find a place at once: a CTA of eight warps each (20 sequences of 300 rows, 8 heads of 256: 8.3 us, with
+    // four warps 8.4; 4 of 500, 40 heads of 128: 7.1, 8.6), else four (60 of 1000, 10 heads of 64: 11.8, with eight 14.0).  A pair
+    // in many pieces: its dims are cut into CTAs of 32, if all of these find a place (one of 30000 rows, 8 heads of 256: 20, not
+    // cut 44; of 131071, 32 heads of 128: 92, 95; 4 of 2000, 16 heads: 10.6, but 10.3), whose warps read twenty pieces at once, or
+    // ten, which takes fewer registers, where the CTAs that count weights are more than find a place beside them (131071: 111, 106).
+    const uint32_t pieces = kAttnWarps * min(tiles, a.ctas / pairs + 2u), places = 2u * (uint32_t)ctx->sm_count;
+    const uint64_t heads = (uint64_t)a.heads * a.n_seq;
+    const bool cut = pieces > 64u && heads * (HD / 32) <= places, wide = cut || heads <= 2u * places;
+    const uint32_t rows = kCountEach * 32u * (wide ? 8u : 4u), count = a.w_out ? a.kv_heads * ((a.cap + rows - 1) / rows) : 0u;
+    const dim3 grid(a.heads * (cut ? HD / 32 : 1) + count, a.n_seq);
+    return cut && (uint64_t)grid.x * a.n_seq <= places
+               ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 8, 20>, grid, dim3(256), 0, a)
+           : cut  ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, 32, 8, 10>, grid, dim3(256), 0, a)
+           : wide ? tm_launch_pdl(ctx, attention_paged_join_kernel<HD, HD, 8, 3>, grid, dim3(256), 0, a)
+                  : tm_launch_pdl(ctx, attention_paged_join_kernel<HD, HD, 4, 2>, grid, dim3(128), 0, a);
 }
 
 // ---- copies between dense planes and pages ---------------------------------------------------------
