@@ -180,6 +180,21 @@ CASES = [
     ([(i * 53) % 150 for i in range(40)], 8, 1, 256, 16, {"window": 70}),
     ([(i * 11) % 90 for i in range(80)], 4, 4, 32, 16, {}),
     ([(i * 29) % 300 for i in range(160)], 2, 2, 64, 64, {"dropped": 5}),
+    # more heads in all than find a place at once
+    ([(i * 37) % 70 for i in range(75)], 8, 4, 32, 16, {}),
+    ([(i * 37) % 90 for i in range(75)], 8, 2, 64, 32, {}),
+    ([(i * 41) % 90 for i in range(75)], 8, 1, 128, 16, {}),
+    ([(i * 43) % 70 for i in range(75)], 8, 2, 256, 16, {}),
+    # pairs in many pieces
+    ([1300], 4, 2, 32, 16, {}),
+    ([1290, 30], 4, 1, 64, 16, {}),
+    ([1500], 6, 2, 256, 64, {"dropped": 40}),
+]
+LONG = [  # pairs in many pieces, and many stretches of weights
+    ([38000], 8, 8, 32, 256),
+    ([38000], 16, 8, 64, 128),
+    ([37000], 8, 8, 128, 64),
+    ([31000], 8, 8, 256, 256),
 ]
 
 
@@ -212,6 +227,16 @@ def test_attention_weights_are_counted(ctx, lens, heads, kvh, hd, page, more):
     t.call(None, w_out)  # from zero
     ctx.fence()
     t.check(np.zeros_like(t.w_in), f32(w_out, t.w_in.shape), held)
+
+
+@pytest.mark.parametrize("lens,heads,kvh,hd,page", LONG)
+def test_attention_weights_of_long_sequences(ctx, lens, heads, kvh, hd, page):
+    t = Paged(ctx, lens, heads, kvh, hd, page, weights=True)
+    held = np.full(t.w_in.shape, 0.25, np.float32)
+    w_in, w_out = ctx.from_array(t.w_in), ctx.from_array(held)
+    t.call(w_in, w_out)
+    ctx.fence()
+    t.check(t.w_in, f32(w_out, t.w_in.shape), held)
 
 
 def test_scale_of_either_sign_and_zero(ctx):
