@@ -593,6 +593,9 @@ def test_copy_refusals(ctx):
         with pytest.raises(cuda.CudaError) as e:
             call(**over)
         assert e.value.code in (-4, -5), over
+    for runs in ([(0, 0, 5)], [(0, 0, 0, 5), (1, 1)]):
+        with pytest.raises(ValueError):
+            call(runs=runs)
     call(runs=[(0, 0, 0, 5), (0, 1, 4, 2)])  # one dense row into two sequences is fine
     ctx.fence()
 

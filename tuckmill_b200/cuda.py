@@ -10,6 +10,8 @@ fails loudly when ``libtm_cuda.so`` has not been built.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from itertools import chain
 from pathlib import Path
 
 import numpy as np
@@ -534,10 +536,12 @@ class CudaContext:
     def kv_pages_copy(self, k_cache, v_cache, k_pages, v_pages, table, status, pages, page_rows, max_pages, kv_heads,
                       head_dim, cap, to_pages, runs):
         """`runs`: (dense sequence, table row, first row, rows) of each run of rows."""
-        flat = [int(u) for seq, at, first, rows in runs for u in (seq, at, first, rows)]
+        flat = array("I", chain.from_iterable(runs))  # 48 runs: 6 us, as a list of ints 35
+        if len(flat) != 4 * len(runs):
+            raise ValueError("a run is (dense sequence, table row, first row, rows)")
         self._call("kv_pages_copy_f16", k_cache.handle, v_cache.handle, k_pages.handle, v_pages.handle, table.handle,
                    status.handle, pages, page_rows, max_pages, kv_heads, head_dim, cap, int(to_pages), len(runs),
-                   (C.c_uint32 * len(flat))(*flat))
+                   (C.c_uint32 * len(flat)).from_buffer(flat))
 
     def kv_pages_evict(self, k_pages, v_pages, table, to_table, len_buf, len_out, weights, weights_out, kept, status,
                        n_seq, kv_heads, head_dim, pages, page_rows, max_pages, keep, first, recent):
