@@ -154,27 +154,88 @@ def _context():
 
 
 class _DeviceArray:
-    """A library buffer as torch sees it."""
+    """A library buffer as torch sees it; once neither a state nor a result holds it, it is there for the next one."""
 
     _KINDS = {torch.float32: "<f4", torch.float16: "<f2", torch.int32: "<i4"}
 
-    def __init__(self, buf, like):
-        self._buf = buf  # keeps the storage
-        self.__cuda_array_interface__ = {"shape": tuple(like.shape), "typestr": self._KINDS[like.dtype],
-                                         "data": (buf.device_ptr(), False), "version": 3}
+    def __init__(self, storage, shape, dtype):
+        self._storage = storage
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": self._KINDS[dtype],
+                                         "data": (storage.at, False), "version": 3}
+
+    def __del__(self):
+        _give(self._storage)
+
+
+# A program keeps its caches, tables and workspaces and fills them again.  So buffers that a state has given up are kept, by
+# their size, for the next state of the same case, as torch keeps the storage of its tensors; every tensor in them is
+# filled anew, and a workspace needs no filling.
+_SPARE = {}
+_SPARE_OF = []
+
+
+class _Storage:
+    def __init__(self, nbytes):
+        self.bytes, self.b = nbytes, _context().buffer(nbytes)
+        self.at = self.b.device_ptr()
+
+
+def _take(nbytes):
+    spare = _SPARE.get(nbytes)
+    return spare.pop() if spare else _Storage(nbytes)
+
+
+def _give(storage):
+    _SPARE.setdefault(storage.bytes, []).append(storage)
+
+
+def _keep_buffers_of(case):
+    torch.cuda.synchronize()  # whatever used the spare buffers has ended
+    if _SPARE_OF != [case]:
+        _SPARE.clear()
+        _SPARE_OF[:] = [dict(case)]
+
+
+class _Workspace:
+    """A buffer that no tensor lies in."""
+
+    def __init__(self, nbytes):
+        self._storage = _take(nbytes)
+        self.b = self._storage.b
+
+    def __del__(self):
+        _give(self._storage)
 
 
 class _Held:
-    """A tensor, and the library's buffer that it lies in where a caller of the library made it."""
+    """A tensor of `values`, or one that `fill` writes; where a caller of the library makes it, it lies in the library's
+    buffer `b`."""
 
-    def __init__(self, t):
-        self.t, self.b = t, None
+    def __init__(self, values=None, shape=None, dtype=None, fill=None):
+        if values is not None:
+            shape, dtype = values.shape, values.dtype
+        self.b = None
         if own:
-            ctx = _context()
-            self.b = ctx.buffer(max(t.numel() * t.element_size(), 4))
-            if t.numel():
-                self.t = torch.as_tensor(_DeviceArray(self.b, t), device=_DEV)
-                self.t.copy_(t)
+            storage = _take(math.prod(shape) * dtype.itemsize)
+            self.b, self.t = storage.b, torch.as_tensor(_DeviceArray(storage, shape, dtype), device=_DEV)
+            if values is not None:
+                self.t.copy_(values)
+        else:
+            self.t = torch.empty(shape, dtype=dtype, device=_DEV) if values is None else values.to(_DEV)
+        if fill:
+            fill(self.t)
+
+
+def _normal(g, *shape, dtype=torch.float32, std=1.0):
+    return _Held(shape=shape, dtype=dtype, fill=lambda t: t.normal_(std=std, generator=g))
+
+
+def _held_words(values):
+    return _Held(torch.tensor(values, dtype=torch.int32))
+
+
+def _zeros(*shape, dtype=torch.float32):
+    return _Held(shape=shape, dtype=dtype, fill=lambda t: t.zero_())
 
 
 def _gen(seed):
@@ -208,11 +269,13 @@ def _tables(g, max_pages, need, pages, sets=1):
 
 
 def _pool(g, case, pages):
-    return torch.randn(pages, case["kv_heads"], case["page"], case["head_dim"], dtype=torch.float16, device=_DEV, generator=g)
+    return _normal(g, pages, case["kv_heads"], case["page"], case["head_dim"], dtype=torch.float16)
 
 
 def prepare(case, seed):
     g = _gen(seed)
+    if own:
+        _keep_buffers_of(case)
     state = {"attention": _prepare_attention, "evict": _prepare_evict, "copy": _prepare_copy,
              "choose": _prepare_choose}[case["kind"]](case, g)
     state["case"] = case
@@ -231,24 +294,24 @@ def _prepare_attention(case, g):
         gone = torch.clamp(_words(lens) + 1 - case["window"], min=0) // case["page"]
         table = torch.where(torch.arange(max_pages, device=_DEV)[None, :] < gone[:, None], torch.full_like(table, _NONE), table)
     st = {
-        "qkv": _Held(torch.randn(s, (heads + 2 * kvh) * hd, device=_DEV, generator=g)),
+        "qkv": _normal(g, s, (heads + 2 * kvh) * hd),
         "q_norm": _Held(1 + 0.1 * torch.randn(hd, device=_DEV, generator=g)),
         "k_norm": _Held(1 + 0.1 * torch.randn(hd, device=_DEV, generator=g)),
         "inv_freq": _Held(_inv_freq(case["n_rot"])),
-        "k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)),
-        "table": _Held(table), "lens": _Held(_words(lens)), "pos": _Held(_words([n + case["dropped"] for n in lens])),
-        "out": _Held(torch.zeros(s, heads * hd, device=_DEV)), "status": _Held(_words([0])),
+        "k": _pool(g, case, pages), "v": _pool(g, case, pages),
+        "table": _Held(table), "lens": _held_words(lens), "pos": _held_words([n + case["dropped"] for n in lens]),
+        "out": _zeros(s, heads * hd), "status": _zeros(1, dtype=torch.int32),
         "max_pages": max_pages, "pages": pages,
     }
     if case["weights"]:  # what earlier tokens gave to each cached row
         before = torch.rand(s, kvh, max_pages * case["page"], device=_DEV, generator=g).pow(4)
-        st["weights"], st["weights_out"] = _Held(before), _Held(torch.zeros_like(before))
+        st["weights"], st["weights_out"] = _Held(before), _zeros(*before.shape)
     if own:
         from tuckmill_b200 import cuda
-        ctx, n = _context(), st["qkv"].b.len()
+        n = st["qkv"].b.len()
         off = [0, heads * hd * 4, (heads + kvh) * hd * 4]
         st["views"] = [st["qkv"].b.view(o, n - o) for o in off]
-        st["scratch"] = ctx.buffer(cuda.attention_paged_scratch_bytes(s, heads, kvh, hd, case["page"], max_pages,
+        st["scratch"] = _Workspace(cuda.attention_paged_scratch_bytes(s, heads, kvh, hd, case["page"], max_pages,
                                                                       case["weights"]))
     return st
 
@@ -256,7 +319,7 @@ def _prepare_attention(case, g):
 def _inv_freq(n_rot):
     """Rotation frequencies of base 1e6, rounded to f32 once."""
     f = 1e6 ** (-np.arange(n_rot // 2, dtype=np.float64) * 2 / n_rot)
-    return torch.from_numpy(f.astype(np.float32)).to(_DEV)
+    return torch.from_numpy(f.astype(np.float32))
 
 
 def _prepare_evict(case, g):
@@ -267,10 +330,10 @@ def _prepare_evict(case, g):
     cap = max_pages * case["page"]
     weights = torch.rand(s, kvh, cap, device=_DEV, generator=g).pow(8)  # a few rows draw most of the attention
     weights = torch.where(weights < 1e-6, torch.zeros_like(weights), weights)  # rows never looked at tie
-    return {"k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)), "table": _Held(table), "to": _Held(to),
-            "lens": _Held(_words(lens)), "lens_out": _Held(_words([0] * s)), "weights": _Held(weights),
-            "weights_out": _Held(torch.zeros_like(weights)), "status": _Held(_words([0])),
-            "kept": _Held(torch.zeros(s, kvh, keep, dtype=torch.int32, device=_DEV)), "max_pages": max_pages, "pages": pages}
+    return {"k": _pool(g, case, pages), "v": _pool(g, case, pages), "table": _Held(table), "to": _Held(to),
+            "lens": _held_words(lens), "lens_out": _zeros(s, dtype=torch.int32), "weights": _Held(weights),
+            "weights_out": _zeros(*weights.shape), "status": _zeros(1, dtype=torch.int32),
+            "kept": _zeros(s, kvh, keep, dtype=torch.int32), "max_pages": max_pages, "pages": pages}
 
 
 def _prepare_copy(case, g):
@@ -281,9 +344,9 @@ def _prepare_copy(case, g):
     cap = max(lens)
     # every other sequence carries on from a third of its length
     runs = [(i, i, n // 3 if i % 2 else 0, n - (n // 3 if i % 2 else 0)) for i, n in enumerate(lens)]
-    dense = lambda: torch.randn(s, kvh, cap, hd, dtype=torch.float16, device=_DEV, generator=g)  # noqa: E731
-    return {"k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)), "kc": _Held(dense()), "vc": _Held(dense()),
-            "table": _Held(table), "status": _Held(_words([0])), "runs": runs, "runs_dev": _words(runs).long(),
+    dense = lambda: _normal(g, s, kvh, cap, hd, dtype=torch.float16)  # noqa: E731
+    return {"k": _pool(g, case, pages), "v": _pool(g, case, pages), "kc": dense(), "vc": dense(),
+            "table": _Held(table), "status": _zeros(1, dtype=torch.int32), "runs": runs, "runs_dev": _words(runs).long(),
             "rows": sum(r[3] for r in runs), "cap": cap, "max_pages": max_pages, "pages": pages}
 
 
@@ -299,13 +362,13 @@ def _prepare_choose(case, g):
     log = torch.where(half, torch.gather(common, 1, pick), rare).to(torch.int32)
     pen = torch.stack([1 + 0.3 * torch.rand(r, device=_DEV, generator=g), 0.5 * torch.rand(r, device=_DEV, generator=g),
                        0.2 * torch.rand(r, device=_DEV, generator=g)], 1)
-    st = {"x": _Held(4 * torch.randn(r, n, device=_DEV, generator=g)), "y": _Held(torch.zeros(r, n, device=_DEV)),
-          "log": _Held(log), "pos": _Held(_words([v - 1 for v in hist])), "prompt": _Held(_words([v // 2 for v in hist])),
+    st = {"x": _normal(g, r, n, std=4.0), "y": _zeros(r, n),
+          "log": _Held(log), "pos": _held_words([v - 1 for v in hist]), "prompt": _held_words([v // 2 for v in hist]),
           "pen": _Held(pen.contiguous()), "stride": stride}
     if nb:
         st["bias_ids"] = _Held(torch.randint(0, n, (r, nb), device=_DEV, generator=g).to(torch.int32))
         st["bias"] = _Held(3 * torch.randn(r, nb, device=_DEV, generator=g))
-        st["bias_n"] = _Held(_words([max(0, nb - 3 * (i % 5)) for i in range(r)]))
+        st["bias_n"] = _held_words([max(0, nb - 3 * (i % 5)) for i in range(r)])
     if case["mask"]:
         words = -(-n // 32)
         # a grammar allows a few tokens in some states and almost all of them inside a string
@@ -315,7 +378,7 @@ def _prepare_choose(case, g):
         st["mask"] = _Held(torch.where(wide, torch.full_like(few, -1), few).to(torch.int32))
     if own:
         from tuckmill_b200 import cuda
-        st["partial"] = _context().buffer(r * cuda.LOGITS_PARTIAL_BYTES)
+        st["partial"] = _Workspace(r * cuda.LOGITS_PARTIAL_BYTES)
     return st
 
 
@@ -348,7 +411,7 @@ def _run_attention(st):
         q, k, v = st["views"]
         width = (heads + 2 * kvh) * hd
         st["ctx"].attention_decode_paged(q, k, v, st["q_norm"].b, st["k_norm"].b, st["inv_freq"].b, st["k"].b, st["v"].b,
-                                         st["table"].b, st["out"].b, st["scratch"], st["pos"].b, st["lens"].b,
+                                         st["table"].b, st["out"].b, st["scratch"].b, st["pos"].b, st["lens"].b,
                                          st["status"].b, s, heads, kvh, hd, c["n_rot"], st["pages"], page, st["max_pages"],
                                          c["window"], 1e-6, scale, q_stride=width, kv_stride=width,
                                          weights_in=w_in.b if w_in else None, weights_out=w_out.b if w_out else None)
@@ -435,7 +498,7 @@ def _run_choose(st):
     if own:
         st["ctx"].logits_adjust_rows(st["x"].b, st["y"].b, r, n, st["log"].b, stride, 1, st["pos"].b, st["pen"].b,
                                      prompt_len=st["prompt"].b, bias_ids=get("bias_ids"), bias_values=get("bias"),
-                                     bias_count=get("bias_n"), bias_cap=c["biases"], mask=get("mask"), partial=st["partial"])
+                                     bias_count=get("bias_n"), bias_cap=c["biases"], mask=get("mask"), partial=st["partial"].b)
         return result
     x, log = st["x"].t, st["log"].t.long().clamp(min=0)
     end, start = st["pos"].t.long()[:, None] + 1, st["prompt"].t.long()[:, None]
