@@ -687,9 +687,9 @@ int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows);
  * weights_in (NULL: zeros; may be weights_out) plus the sum of the softmax weights that the KV head's query heads give it
  * now.  The new row starts from 0; entries behind it are left as they are.
  * A length of TM_CUDA_SEQ_NONE: the sequence takes no part, nothing of it is written.  A length >= max_pages * page_rows:
- * the same, and bit 0 of status[0] is set.  An infinity or NaN in a row in sight makes the heads that read it NaN; rows out
- * of sight have no effect.  scratch holds tm_cuda_attention_paged_scratch_bytes and needs no clearing; calls that share it
- * must be ordered on the stream. */
+ * the same, and bit 0 of status[0] is set.  An infinity or NaN in a key in sight makes the heads that read it, and the weights
+ * that they count, NaN; one in a value makes its dimension of their outputs NaN; rows out of sight have no effect.  scratch
+ * holds tm_cuda_attention_paged_scratch_bytes and needs no clearing; calls that share it must be ordered on the stream. */
 size_t tm_cuda_attention_paged_scratch_bytes(uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                              uint32_t page_rows, uint32_t max_pages, int weights);
 int tm_cuda_attention_decode_paged_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *q, tm_cuda_buffer *k, tm_cuda_buffer *v,

@@ -260,6 +260,35 @@ def test_queries_of_any_size(ctx):
         t.check()
 
 
+@pytest.mark.parametrize("hd,heads,kvh,more", [(32, 8, 2, {}), (64, 16, 1, {"window": 150}), (128, 8, 2, {}), (256, 12, 4, {})])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_infinities_and_nan_in_sight(ctx, hd, heads, kvh, more, bad):
+    """One in a key makes NaN of the heads that read it and of the weights that they count, one in a value of its own
+    dimension of their outputs; all else has the bits that it has without."""
+    group = heads // kvh
+    for of_key in (True, False):
+        t = Paged(ctx, [200, 70, 3], heads, kvh, hd, 16, weights=True, seed=13, **more)
+        w_in, w_out = ctx.from_array(t.w_in), ctx.from_array(np.zeros_like(t.w_in))
+        t.call(w_in, w_out)
+        ctx.fence()
+        t.check(t.w_in, f32(w_out, t.w_in.shape), np.zeros_like(t.w_in))
+        want, want_w = f32(t.bout, t.out0.shape).copy().reshape(3, heads, hd), f32(w_out, t.w_in.shape).copy()
+        for s, h, j, d in ((0, 0, 137, 5), (1, kvh - 1, 69, hd - 1), (2, 0, 0, 0)):
+            t.k[t.table[s, j // 16], h, j % 16, d] = bad if of_key else t.k[t.table[s, j // 16], h, j % 16, d]
+            t.v[t.table[s, j // 16], h, j % 16, d] = t.v[t.table[s, j // 16], h, j % 16, d] if of_key else bad
+            if of_key:
+                want[s, h * group:(h + 1) * group] = np.nan
+                want_w[s, h, t.start(s):t.lens[s] + 1] = np.nan
+            else:
+                want[s, h * group:(h + 1) * group, d] = np.nan
+        t.bk.upload(0, t.k)
+        t.bv.upload(0, t.v)
+        t.call(w_in, w_out)
+        ctx.fence()
+        np.testing.assert_array_equal(f32(t.bout, t.out0.shape).reshape(want.shape), want)
+        np.testing.assert_array_equal(f32(w_out, t.w_in.shape), want_w)
+
+
 def test_a_full_sequence_and_a_bad_page(ctx):
     t = Paged(ctx, [64, 30, 20], 4, 2, 64, 16, max_pages=4, seed=7)
     t.call()

@@ -404,8 +404,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             // rows j0 + g and j0 + g + 8, heads 2t and 2t + 1
             const uint32_t ja = j0 + g, jb = ja + 8u;
             const bool see_a = ja >= start && ja <= len, see_b = jb >= start && jb <= len;
-            const float s0 = see_a ? (hi[0] + lo[0]) * f0 : -INFINITY, s1 = see_a ? (hi[1] + lo[1]) * f1 : -INFINITY;
-            const float s2 = see_b ? (hi[2] + lo[2]) * f0 : -INFINITY, s3 = see_b ? (hi[3] + lo[3]) * f1 : -INFINITY;
+            // (z - z: an infinity is a NaN from here on.  Only an infinite key makes one, and with which sign would hang on how the
+            // query was split.)
+            auto score = [](float z, float f) { return fmaf(z, f, z - z); };
+            const float s0 = see_a ? score(hi[0] + lo[0], f0) : -INFINITY, s1 = see_a ? score(hi[1] + lo[1], f1) : -INFINITY;
+            const float s2 = see_b ? score(hi[2] + lo[2], f0) : -INFINITY, s3 = see_b ? score(hi[3] + lo[3], f1) : -INFINITY;
             if (scores) {
                 float *row = scores + (size_t)ja * a.group;
                 if (see_a && 2 * t < heads) row[0] = s0;
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(c
                 l += sl[x];
                 o += so[x][d];
             }
-            a.out[((size_t)s * a.heads + head) * HD + d0 + d] = o / l;
+            a.out[((size_t)s * a.heads + head) * HD + d0 + d] = o / l + (o - o);  // (NaN of an infinite value, as of a key)
         }
         return;
     }
