@@ -289,6 +289,20 @@ def test_infinities_and_nan_in_sight(ctx, hd, heads, kvh, more, bad):
         np.testing.assert_array_equal(f32(w_out, t.w_in.shape), want_w)
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_small_elements_of_a_query_beside_large_ones(ctx, hd):
+    """Two elements of every query are 2^14 times the others, and meet zeros in every key: the small ones alone make the
+    scores."""
+    t = Paged(ctx, [3, 200], 4, 2, hd, 16, n_rot=2, seed=14)
+    t.qn[:2], t.kn[:2] = 2.0 ** 14, 0
+    t.k[..., :2] = 0
+    for b, x in ((t.bqn, t.qn), (t.bkn, t.kn), (t.bk, t.k)):
+        b.upload(0, x)
+    t.call()
+    ctx.fence()
+    t.check()
+
+
 def test_a_full_sequence_and_a_bad_page(ctx):
     t = Paged(ctx, [64, 30, 20], 4, 2, 64, 16, max_pages=4, seed=7)
     t.call()

@@ -70,12 +70,15 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // rows as the 16-row operand and the heads as the 8 columns: S^T = K Q^T, then O^T = V^T P^T, with P transposed in registers.
 //
 // Accuracy: cached rows are f16, so their products with f16 operands are exact in f32.  Q and P are split into a sum of two
-// f16 each (22 bits; Q against a power of two at its largest element, P in units of 2^-14, so that neither runs out of
-// exponents), and every product of a 16-row step starts from zero and is added to the f32 sums by a fused multiply-add:
-// results are those of 32-bit arithmetic.  The second multiply hides behind the loads.
+// f16 each (22 bits; Q against a power of two at its largest element, P in units of 2^-14), and every product of a 16-row
+// step starts from zero and is added to the f32 sums by a fused multiply-add: results are those of 32-bit arithmetic.  What
+// the first f16 leaves of an element of Q is multiplied by 2^12, or it would lie among the subnormals: an element is off by at
+// most 2^-37 of the largest where it would be 2^-25, which a large key beside a small element shows (the sums of both parts are
+// apart, so this costs nothing).  The second multiply hides behind the loads.
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr uint32_t kBlock = 16, kTile = kBlock * kAttnWarps;
 constexpr float kUnit = 14.0f;  // P and its sums are held times 2^14
+constexpr float kLow = 4096.0f;  // the second f16 of a query element is held times 2^12
 
 template <int HD>
 struct attn_cfg {
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
     for (int r = 0; r < EPL; ++r) top = fmaxf(top, fabsf(row[lane + 32 * r]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // q = 2^e (hi + lo), |hi| < 2; a vector of zeros, infinities or NaN keeps e = 0
+    // q = 2^e (hi + lo / kLow), |hi| < 2; a vector of zeros, infinities or NaN keeps e = 0
     int e = (int)((__float_as_uint(top) >> 23) & 0xffu) - 127;
     e = top > 0.0f && top < INFINITY ? max(-120, min(120, e)) : 0;
     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -263,7 +266,8 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
         const __half2 h0 = __floats2half2_rn(z0, z1), h1 = __floats2half2_rn(z2, z3);
         const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
         a.ops[(pair * (HD / 16) + i / 4u) * 32 + h * 4u + i % 4u] =
-            make_uint4(bits(h0), bits(h1), bits(__floats2half2_rn(z0 - f0.x, z1 - f0.y)), bits(__floats2half2_rn(z2 - f1.x, z3 - f1.y)));
+            make_uint4(bits(h0), bits(h1), bits(__floats2half2_rn((z0 - f0.x) * kLow, (z1 - f0.y) * kLow)),
+                       bits(__floats2half2_rn((z2 - f1.x) * kLow, (z3 - f1.y) * kLow)));
     }
 }
 
@@ -407,8 +411,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             // (z - z: an infinity is a NaN from here on.  Only an infinite key makes one, and with which sign would hang on how the
             // query was split.)
             auto score = [](float z, float f) { return fmaf(z, f, z - z); };
-            const float s0 = see_a ? score(hi[0] + lo[0], f0) : -INFINITY, s1 = see_a ? score(hi[1] + lo[1], f1) : -INFINITY;
-            const float s2 = see_b ? score(hi[2] + lo[2], f0) : -INFINITY, s3 = see_b ? score(hi[3] + lo[3], f1) : -INFINITY;
+            float z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = fmaf(lo[i], 1.0f / kLow, hi[i]);
+            const float s0 = see_a ? score(z[0], f0) : -INFINITY, s1 = see_a ? score(z[1], f1) : -INFINITY;
+            const float s2 = see_b ? score(z[2], f0) : -INFINITY, s3 = see_b ? score(z[3], f1) : -INFINITY;
             if (scores) {
                 float *row = scores + (size_t)ja * a.group;
                 if (see_a && 2 * t < heads) row[0] = s0;
