@@ -303,6 +303,24 @@ def test_small_elements_of_a_query_beside_large_ones(ctx, hd):
     t.check()
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("octaves", [24.4, 30.7, 37.3])
+def test_small_weights_beside_a_large_one(ctx, hd, octaves):
+    """One row weighs 2^octaves times each of the others and its value is zero: the small weights alone make the output."""
+    t = Paged(ctx, [300], 1, 1, hd, 16, n_rot=2, seed=15)
+    q = t.turned(t.qkv[0, :hd].reshape(1, hd), t.qn, t.pos[0])[0][0]
+    t.kn[:] = 0
+    for j in range(300):
+        t.k[t.table[0, j // 16], 0, j % 16] = 0
+    t.k[t.table[0, 0], 0, 7] = octaves * np.log(2) / float(t.scale) / (q @ q) * q
+    t.v[t.table[0, 0], 0, 7] = 0
+    for b, x in ((t.bkn, t.kn), (t.bk, t.k), (t.bv, t.v)):
+        b.upload(0, x)
+    t.call()
+    ctx.fence()
+    t.check()
+
+
 def test_a_full_sequence_and_a_bad_page(ctx):
     t = Paged(ctx, [64, 30, 20], 4, 2, 64, 16, max_pages=4, seed=7)
     t.call()

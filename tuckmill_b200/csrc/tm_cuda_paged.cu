@@ -72,13 +72,15 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // Accuracy: cached rows are f16, so their products with f16 operands are exact in f32.  Q and P are split into a sum of two
 // f16 each (22 bits; Q against a power of two at its largest element, P in units of 2^-14), and every product of a 16-row
 // step starts from zero and is added to the f32 sums by a fused multiply-add: results are those of 32-bit arithmetic.  What
-// the first f16 leaves of an element of Q is multiplied by 2^12, or it would lie among the subnormals: an element is off by at
-// most 2^-37 of the largest where it would be 2^-25, which a large key beside a small element shows (the sums of both parts are
-// apart, so this costs nothing).  The second multiply hides behind the loads.
+// the first f16 leaves is multiplied by 2^12, or it would lie among the subnormals: an element of Q is off by at most 2^-37 of
+// the largest where it would be 2^-25, which a large key beside a small element shows, and a weight by at most 2^-51 of the
+// largest where it would be 2^-39, which a first row that draws all attention and has a value of zero shows.  (Q's parts have
+// sums of their own anyway; for P's apart the rows cost 0.1 us more of 5.4, 22.0 and 8.0, 0.3 of 71.2.)  The second multiply
+// hides behind the loads.
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr uint32_t kBlock = 16, kTile = kBlock * kAttnWarps;
 constexpr float kUnit = 14.0f;  // P and its sums are held times 2^14
-constexpr float kLow = 4096.0f;  // the second f16 of a query element is held times 2^12
+constexpr float kLow = 4096.0f;  // the second f16 of an element of Q or P is held times 2^12
 
 template <int HD>
 struct attn_cfg {
@@ -443,20 +445,20 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
             const __half2 pa = __floats2half2_rn(p0, p1), pb = __floats2half2_rn(p2, p3);
             const float2 fa = __half22float2(pa), fb = __half22float2(pb);
             const uint32_t h0 = transpose8x8(bits(pa)), h1 = transpose8x8(bits(pb));
-            const uint32_t r0 = transpose8x8(bits(__floats2half2_rn(p0 - fa.x, p1 - fa.y)));
-            const uint32_t r1 = transpose8x8(bits(__floats2half2_rn(p2 - fb.x, p3 - fb.y)));
+            const uint32_t r0 = transpose8x8(bits(__floats2half2_rn((p0 - fa.x) * kLow, (p1 - fa.y) * kLow)));
+            const uint32_t r1 = transpose8x8(bits(__floats2half2_rn((p2 - fb.x) * kLow, (p3 - fb.y) * kLow)));
             const uint32_t mat = lane >> 3, vr = (lane & 7u) + (mat >> 1) * 8u;
 #pragma unroll
             for (int mt = 0; mt < KT; ++mt) {
                 uint32_t a0, a1, a2, a3;
                 ldsm_x4_t(vb + sw<PITCH>(vr, mt * 2 + (mat & 1u)), a0, a1, a2, a3);
-                float d[4] = {0, 0, 0, 0};
+                float d[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0};
                 mma_f16(d, a0, a1, a2, a3, h0, h1);
-                mma_f16(d, a0, a1, a2, a3, r0, r1);
-                o[mt][0] = fmaf(o[mt][0], al0, d[0]);
-                o[mt][1] = fmaf(o[mt][1], al1, d[1]);
-                o[mt][2] = fmaf(o[mt][2], al0, d[2]);
-                o[mt][3] = fmaf(o[mt][3], al1, d[3]);
+                mma_f16(e, a0, a1, a2, a3, r0, r1);
+                o[mt][0] = fmaf(o[mt][0], al0, fmaf(e[0], 1.0f / kLow, d[0]));
+                o[mt][1] = fmaf(o[mt][1], al1, fmaf(e[1], 1.0f / kLow, d[1]));
+                o[mt][2] = fmaf(o[mt][2], al0, fmaf(e[2], 1.0f / kLow, d[2]));
+                o[mt][3] = fmaf(o[mt][3], al1, fmaf(e[3], 1.0f / kLow, d[3]));
             }
         }
         // ---- what this warp has found (zeros, where it saw no row) ----
