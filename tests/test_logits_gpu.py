@@ -215,3 +215,22 @@ def test_logits_refusals(ctx):
         assert e.value.code in (-4, -5), over
     call()
     ctx.fence()
+
+
+def test_buffers_of_another_context_are_refused(ctx):
+    """A token log and positions that a call does not use are looked at no further than a buffer of its own, or refused."""
+    other = cuda.CudaContext(0)
+    try:
+        n = 64
+        x, y, mask = ctx.from_array(np.zeros((1, n), np.float32)), ctx.buffer(n * 4), ctx.from_array(np.full(2, 0xFFFFFFFF, np.uint32))
+        own, foreign = ctx.buffer(16), other.buffer(16)
+        for over in (dict(log=foreign), dict(pos_buf=foreign), dict(log=own, pos_buf=foreign), dict(log=foreign, pos_buf=own)):
+            with pytest.raises(cuda.CudaError) as e:
+                ctx.logits_adjust_rows(x, y, 1, n, log_stride=4, mask=mask, **over)
+            assert e.value.code == -5, over
+        ctx.logits_adjust_rows(x, y, 1, n, log=own, log_stride=4, pos_buf=own, mask=mask)
+        ctx.fence()
+        np.testing.assert_array_equal(y.download(0, n * 4, np.float32), np.zeros(n, np.float32))
+        foreign.free()
+    finally:
+        other.close()

@@ -272,6 +272,9 @@ int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_c
         if (partial) TM_CHECK_BUF(log, nlog, "token logs");
         else TM_CHECK_IN(log, nlog, "token logs");
         TM_CHECK_IN(pos_buf, nr, "positions");
+    } else {  // a handle that is not looked at has to be one all the same
+        if (log) TM_CHECK_IN(log, 1, "token logs");
+        if (pos_buf) TM_CHECK_IN(pos_buf, 1, "positions");
     }
     if (penalties) TM_CHECK_IN(penalties, nr * 3, "penalties");
     if (prompt_len) TM_CHECK_IN(prompt_len, nr, "prompt lengths");
@@ -295,8 +298,8 @@ int tm_cuda_logits_adjust_rows_f32_dev(tm_cuda_ctx *ctx, tm_cuda_buffer *x, tm_c
     auto u32 = [](tm_cuda_buffer *b) { return b ? (const uint32_t *)b->dev : nullptr; };
     a.x = (const float *)x->dev;
     a.y = (float *)y->dev;
-    a.log = u32(log);
-    a.pos = u32(pos_buf);
+    a.log = u32(uses_log ? log : nullptr);
+    a.pos = u32(uses_log ? pos_buf : nullptr);
     a.prompt = u32(prompt_len);
     a.bias_ids = u32(bias_ids);
     a.bias_count = u32(bias_count);
