@@ -32,3 +32,9 @@ def test_no_context_is_refused(name, args):
     err = C.create_string_buffer(128)
     assert getattr(cuda.load_library(), "tm_cuda_" + name)(None, *args, err, 128) == -5
     assert b"context" in err.value
+
+
+@pytest.mark.parametrize("runs", [[(0, 0, 5)], [(0, 0, 0, 5), (1, 1)], [(0, 0, 0), (5, 1, 1, 0, 2)], [(), (0, 0, 0, 5, 1, 1, 0, 2)]])
+def test_runs_of_a_page_copy_are_four_numbers_each(runs):
+    with pytest.raises(ValueError):
+        cuda.CudaContext.kv_pages_copy(None, None, None, None, None, None, None, 1, 16, 1, 1, 64, 16, True, runs)

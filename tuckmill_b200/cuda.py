@@ -536,9 +536,9 @@ class CudaContext:
     def kv_pages_copy(self, k_cache, v_cache, k_pages, v_pages, table, status, pages, page_rows, max_pages, kv_heads,
                       head_dim, cap, to_pages, runs):
         """`runs`: (dense sequence, table row, first row, rows) of each run of rows."""
-        flat = array("I", chain.from_iterable(runs))  # 48 runs: 6 us, as a list of ints 35
-        if len(flat) != 4 * len(runs):
+        if set(map(len, runs)) - {4}:
             raise ValueError("a run is (dense sequence, table row, first row, rows)")
+        flat = array("I", chain.from_iterable(runs))  # 48 runs, with the line above: 7.5 us, as a list of ints 35
         self._call("kv_pages_copy_f16", k_cache.handle, v_cache.handle, k_pages.handle, v_pages.handle, table.handle,
                    status.handle, pages, page_rows, max_pages, kv_heads, head_dim, cap, int(to_pages), len(runs),
                    (C.c_uint32 * len(flat)).from_buffer(flat))
