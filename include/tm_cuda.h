@@ -685,7 +685,8 @@ int tm_cuda_kv_pages_supported(uint32_t head_dim, uint32_t page_rows);
  * 64 rows, of every KV head and eight of its query heads, are fewer than 2^32.
  * weights_out (may be NULL): [n_seq][kv_heads][max_pages * page_rows] f32, the attention that each row has drawn:
  * weights_in (NULL: zeros; may be weights_out) plus the sum of the softmax weights that the KV head's query heads give it
- * now.  The new row starts from 0; entries behind it are left as they are.
+ * now.  The new row starts from 0; entries behind it are left as they are.  The scratch then holds a score for every row of
+ * max_pages pages and every head, and the time grows with max_pages too, however few rows the sequences have.
  * A length of TM_CUDA_SEQ_NONE: the sequence takes no part, nothing of it is written.  A length >= max_pages * page_rows:
  * the same, and bit 0 of status[0] is set.  An infinity or NaN in a key in sight makes the heads that read it, and the weights
  * that they count, NaN; one in a value makes its dimension of their outputs NaN; rows out of sight have no effect.  scratch
@@ -717,7 +718,9 @@ int tm_cuda_kv_pages_copy_f16(tm_cuda_ctx *ctx, tm_cuda_buffer *k_cache, tm_cuda
  * sequence with at most keep rows keeps all of them: kept[s][h][i] = i below its length and 0xFFFFFFFF behind.
  * to_table is `table` itself (the rows move down in place; no page may then be shared) or names pages that no
  * sequence reads from.  A length of TM_CUDA_SEQ_NONE, or one > max_pages * page_rows (which sets bit 0 of
- * status[0]): nothing of the sequence is written, len_out receives the length as it is. */
+ * status[0]): nothing of the sequence is written, len_out receives the length as it is.  From then on rows are fewer than
+ * positions: tm_cuda_attention_prefill, which has one number for both, does not serve the sequence any more, and further
+ * tokens go one by one through tm_cuda_attention_decode_paged_dev. */
 int tm_cuda_kv_pages_evict(tm_cuda_ctx *ctx, tm_cuda_buffer *k_pages, tm_cuda_buffer *v_pages, tm_cuda_buffer *table,
                            tm_cuda_buffer *to_table, tm_cuda_buffer *len_buf, tm_cuda_buffer *len_out,
                            tm_cuda_buffer *weights, tm_cuda_buffer *weights_out, tm_cuda_buffer *kept,

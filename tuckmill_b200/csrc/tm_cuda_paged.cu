@@ -54,14 +54,15 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // One new token of every sequence: z_hj = scale q_h . k_j over the rows j in sight, P = softmax(z), out_h = sum_j P_hj v_j,
 // and, where a caller counts attention, weights[kv][j] += sum over the group's heads of P_hj.
 //
-// What bounds it: the cached rows' bytes, 4 head_dim per row and KV head.  So every row is read once for all (up to
-// eight) query heads of its group, and the machine's bandwidth is shared out evenly however ragged the lengths are:
+// What bounds it: the cached rows' bytes, 4 head_dim per row and KV head.  So every row is read once for eight query heads
+// of its group (with more, a pair for every eight of them, each of which reads the rows again: 32 sequences of up to 4000 rows, one
+// KV head of 128, 8 query heads 15 us, 32 heads 28), and the machine's bandwidth is shared out evenly however ragged the lengths are:
 // the tiles of 64 rows of all (sequence, KV head) pairs form one line, and CTA i of G takes the i-th of G equal runs of
 // it.  Three launches: the vectors (queries and new rows: norm, rotation, f16), the rows, and the join of what the warps
 // have found.  The second starts beside the first and waits for it when it has its rows on their way.
 //
-// What it measured (8 KV heads of 128): the rows of one sequence of 131071 (537 MB) 86 us, 6.2 TB/s, of 32 up to 4095 (343 MB
-// with the scores) 60 us, 5.7 TB/s; around them 3 us until the first rows arrive and 3 to 7 us of the join.  (Slices whose
+// What it measured (8 KV heads of 128): the rows of one sequence of 131071 (537 MB) 84 us, 6.4 TB/s, of 32 up to 4095 (343 MB
+// with the scores) 61 us, 5.7 TB/s; around them 3 us until the first rows arrive and 3 to 7 us of the join.  (Slices whose
 // last eighth went to whichever warp was free measured the same: what ends late waits for the memory, not for work.)
 //
 // A warp takes 16 rows of each tile through its own ring of cp.async stages and keeps its own running (max, sum, output):
@@ -492,7 +493,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_cfg<HD>::kCtas) attention_p
 
 // Joins the warps' pieces of every pair (a CTA takes DIMS of a head, a warp a piece), and counts the attention of stretches
 // of rows (the CTAs behind those).  What needs neither pieces nor scores is done while the rows are still being read, and
-// every warp finds the maximum of all pieces for itself, so that nothing waits for it but the last sums.
+// every warp finds the maximum of all pieces for itself, so that nothing waits for it but the last sums.  (Counting CTAs are as many
+// as rows that the tables have room for; those behind a sequence's last row look at its length and leave: 64 sequences of up to 1000
+// rows, 8 KV heads, tables for 1000 rows 41.5 us, for 16384 62.7, for 131072 205.)
 constexpr uint32_t kCountEach = 4;
 template <int HD, int DIMS, uint32_t kJoinWarps, int kBatch>  // kBatch: pieces of a warp on their way at a time
 __global__ void __launch_bounds__(32 * kJoinWarps) attention_paged_join_kernel(const paged_args a) {
@@ -702,7 +705,8 @@ cudaError_t launch_paged(tm_cuda_ctx *ctx, paged_args a) {
 //
 // Moves 4 head_dim bytes a row and KV head each way and computes nothing: 16 bytes a thread and load, all loads of a
 // thread before its first store.  A CTA takes up to 64 rows of one run, one head, keys or values.  Bound by the memory:
-// 670 MB (32 sequences of up to 4096 rows, 8 heads of 128) 89 us, 7.5 TB/s of reads and writes together.
+// 670 MB (32 sequences of up to 4096 rows, 8 heads of 128) 89 us, 7.5 TB/s of reads and writes together, of which a part is the
+// 126 MB of L2's (a plain copy of 4 GB: 6.5 TB/s).
 constexpr uint32_t kCopyRows = 64, kCopyThreads = 256;
 struct copy_runs {
     uint32_t n;
@@ -826,8 +830,9 @@ __device__ __forceinline__ uint4 ld_rank4(const uint32_t *p, uint32_t rank) {
     return v;
 }
 
-// Of a head's rows this CTA (`rank` of `ctas` in a cluster; MANY: more than one; a rank behind them has none) looks after r0 .. r1.  HELD: their weights stay
-// in registers (at most a stretch of them); else they are read again for every pass, a stretch ahead.
+// Of a head's rows this CTA (`rank` of `ctas` in a cluster; MANY: more than one; a rank behind them has none) looks after
+// r0 .. r1.  HELD: their weights stay in registers (at most a stretch of them); else they are read again for every pass, a
+// stretch ahead.
 constexpr uint32_t kMostCtas = 8;
 template <bool HELD, bool MANY>
 __device__ __forceinline__ void select_rows(const evict_args &a, const float *w, float *w_out, uint32_t *kept, uint32_t len, uint32_t rank,
@@ -1069,7 +1074,9 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const evict
 }
 
 // In place: a CTA takes 64 bytes of every row of a head, so that the columns need not wait for one another, and goes up the
-// rows: what it stores lies at or below what it has read.
+// rows: what it stores lies at or below what it has read.  Bound by the loads' latency, three behind one another a stretch, and with
+// few heads by the few CTAs (the whole eviction, 8 heads of 128, in place and into other pages: one sequence of 1001 rows to 300 9.3
+// and 7.3 us, of 16000 to 8000 109 and 26, 32 of up to 4096 to 2048 112 and 91).
 constexpr uint32_t kShiftEach = 8, kShiftRows = kMoveThreads / 4 * kShiftEach;
 template <int HD>
 __global__ void __launch_bounds__(kMoveThreads) kv_evict_shift_kernel(const evict_args a) {
