@@ -154,88 +154,69 @@ def _context():
 
 
 class _DeviceArray:
-    """A library buffer as torch sees it; once neither a state nor a result holds it, it is there for the next one."""
+    """A library buffer as torch sees it: bytes."""
 
-    _KINDS = {torch.float32: "<f4", torch.float16: "<f2", torch.int32: "<i4"}
-
-    def __init__(self, storage, shape, dtype):
-        self._storage = storage
-        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": self._KINDS[dtype],
-                                         "data": (storage.at, False), "version": 3}
-
-    def __del__(self):
-        _give(self._storage)
-
-
-# A program keeps its caches, tables and workspaces and fills them again.  So buffers that a state has given up are kept, by
-# their size, for the next state of the same case, as torch keeps the storage of its tensors; every tensor in them is
-# filled anew, and a workspace needs no filling.
-_SPARE = {}
-_SPARE_OF = []
+    def __init__(self, buf):
+        self.__cuda_array_interface__ = {"shape": (len(buf),), "typestr": "|u1", "data": (buf.device_ptr(), False), "version": 3}
 
 
 class _Storage:
-    def __init__(self, nbytes):
-        self.bytes, self.b = nbytes, _context().buffer(nbytes)
-        self.at = self.b.device_ptr()
+    """A buffer of the library's.  A program keeps its caches, tables and workspaces and fills them again: so a buffer that
+    no state and no result holds any more serves the next state of its case, as torch does with the storage of its tensors.
+    Every tensor in it is filled anew; a workspace needs no filling."""
 
-
-def _take(nbytes):
-    spare = _SPARE.get(nbytes)
-    return spare.pop() if spare else _Storage(nbytes)
-
-
-def _give(storage):
-    _SPARE.setdefault(storage.bytes, []).append(storage)
-
-
-def _keep_buffers_of(case):
-    torch.cuda.synchronize()  # whatever used the spare buffers has ended
-    if _SPARE_OF != [case]:
-        _SPARE.clear()
-        _SPARE_OF[:] = [dict(case)]
-
-
-class _Workspace:
-    """A buffer that no tensor lies in."""
+    _spare, _used, _of = {}, False, None  # by size; whether one was in use since the last wait; of which case
 
     def __init__(self, nbytes):
-        self._storage = _take(nbytes)
-        self.b = self._storage.b
+        self.b = _context().buffer(nbytes)
+        self.bytes, self.all = nbytes, torch.as_tensor(_DeviceArray(self.b), device=_DEV)
+
+    @classmethod
+    def take(cls, nbytes):
+        spare = cls._spare.get(nbytes)
+        if not spare:
+            return _Lease(cls(nbytes))
+        if cls._used:
+            torch.cuda.synchronize()  # what used the spare buffers has ended
+            cls._used = False
+        return _Lease(spare.pop())
+
+    @classmethod
+    def give(cls, storage):
+        cls._used = True
+        cls._spare.setdefault(storage.bytes, []).append(storage)
+
+    @classmethod
+    def keep_only(cls, case):
+        if cls._of != case:
+            cls._spare.clear()
+            cls._of = dict(case)
+
+
+class _Lease:
+    """Held by whoever uses a storage: a tensor in it, or a state whose workspace it is."""
+
+    def __init__(self, storage):
+        self.storage, self.b = storage, storage.b
+
+    def tensor(self, like):
+        t = self.storage.all.view(like.dtype).view(like.shape)
+        t.lease = self
+        return t
 
     def __del__(self):
-        _give(self._storage)
+        _Storage.give(self.storage)
 
 
 class _Held:
-    """A tensor of `values`, or one that `fill` writes; where a caller of the library makes it, it lies in the library's
-    buffer `b`."""
+    """A tensor, and the library's buffer that it lies in where a caller of the library made it."""
 
-    def __init__(self, values=None, shape=None, dtype=None, fill=None):
-        if values is not None:
-            shape, dtype = values.shape, values.dtype
-        self.b = None
+    def __init__(self, t):
+        self.t, self.b = t, None
         if own:
-            storage = _take(math.prod(shape) * dtype.itemsize)
-            self.b, self.t = storage.b, torch.as_tensor(_DeviceArray(storage, shape, dtype), device=_DEV)
-            if values is not None:
-                self.t.copy_(values)
-        else:
-            self.t = torch.empty(shape, dtype=dtype, device=_DEV) if values is None else values.to(_DEV)
-        if fill:
-            fill(self.t)
-
-
-def _normal(g, *shape, dtype=torch.float32, std=1.0):
-    return _Held(shape=shape, dtype=dtype, fill=lambda t: t.normal_(std=std, generator=g))
-
-
-def _held_words(values):
-    return _Held(torch.tensor(values, dtype=torch.int32))
-
-
-def _zeros(*shape, dtype=torch.float32):
-    return _Held(shape=shape, dtype=dtype, fill=lambda t: t.zero_())
+            lease = _Storage.take(t.numel() * t.element_size())
+            self.b, self.t = lease.b, lease.tensor(t)
+            self.t.copy_(t)
 
 
 def _gen(seed):
@@ -269,18 +250,17 @@ def _tables(g, max_pages, need, pages, sets=1):
 
 
 def _pool(g, case, pages):
-    return _normal(g, pages, case["kv_heads"], case["page"], case["head_dim"], dtype=torch.float16)
+    return torch.randn(pages, case["kv_heads"], case["page"], case["head_dim"], dtype=torch.float16, device=_DEV, generator=g)
 
 
 def prepare(case, seed):
     g = _gen(seed)
-    if own:
-        _keep_buffers_of(case)
     state = {"attention": _prepare_attention, "evict": _prepare_evict, "copy": _prepare_copy,
              "choose": _prepare_choose}[case["kind"]](case, g)
     state["case"] = case
     if own:
         state["ctx"] = _context()
+        _Storage.keep_only(case)
         torch.cuda.synchronize()  # what torch wrote is complete before the library's stream reads it
     return state
 
@@ -294,24 +274,24 @@ def _prepare_attention(case, g):
         gone = torch.clamp(_words(lens) + 1 - case["window"], min=0) // case["page"]
         table = torch.where(torch.arange(max_pages, device=_DEV)[None, :] < gone[:, None], torch.full_like(table, _NONE), table)
     st = {
-        "qkv": _normal(g, s, (heads + 2 * kvh) * hd),
+        "qkv": _Held(torch.randn(s, (heads + 2 * kvh) * hd, device=_DEV, generator=g)),
         "q_norm": _Held(1 + 0.1 * torch.randn(hd, device=_DEV, generator=g)),
         "k_norm": _Held(1 + 0.1 * torch.randn(hd, device=_DEV, generator=g)),
         "inv_freq": _Held(_inv_freq(case["n_rot"])),
-        "k": _pool(g, case, pages), "v": _pool(g, case, pages),
-        "table": _Held(table), "lens": _held_words(lens), "pos": _held_words([n + case["dropped"] for n in lens]),
-        "out": _zeros(s, heads * hd), "status": _zeros(1, dtype=torch.int32),
+        "k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)),
+        "table": _Held(table), "lens": _Held(_words(lens)), "pos": _Held(_words([n + case["dropped"] for n in lens])),
+        "out": _Held(torch.zeros(s, heads * hd, device=_DEV)), "status": _Held(_words([0])),
         "max_pages": max_pages, "pages": pages,
     }
     if case["weights"]:  # what earlier tokens gave to each cached row
         before = torch.rand(s, kvh, max_pages * case["page"], device=_DEV, generator=g).pow(4)
-        st["weights"], st["weights_out"] = _Held(before), _zeros(*before.shape)
+        st["weights"], st["weights_out"] = _Held(before), _Held(torch.zeros_like(before))
     if own:
         from tuckmill_b200 import cuda
         n = st["qkv"].b.len()
         off = [0, heads * hd * 4, (heads + kvh) * hd * 4]
         st["views"] = [st["qkv"].b.view(o, n - o) for o in off]
-        st["scratch"] = _Workspace(cuda.attention_paged_scratch_bytes(s, heads, kvh, hd, case["page"], max_pages,
+        st["scratch"] = _Storage.take(cuda.attention_paged_scratch_bytes(s, heads, kvh, hd, case["page"], max_pages,
                                                                       case["weights"]))
     return st
 
@@ -319,7 +299,7 @@ def _prepare_attention(case, g):
 def _inv_freq(n_rot):
     """Rotation frequencies of base 1e6, rounded to f32 once."""
     f = 1e6 ** (-np.arange(n_rot // 2, dtype=np.float64) * 2 / n_rot)
-    return torch.from_numpy(f.astype(np.float32))
+    return torch.from_numpy(f.astype(np.float32)).to(_DEV)
 
 
 def _prepare_evict(case, g):
@@ -330,10 +310,10 @@ def _prepare_evict(case, g):
     cap = max_pages * case["page"]
     weights = torch.rand(s, kvh, cap, device=_DEV, generator=g).pow(8)  # a few rows draw most of the attention
     weights = torch.where(weights < 1e-6, torch.zeros_like(weights), weights)  # rows never looked at tie
-    return {"k": _pool(g, case, pages), "v": _pool(g, case, pages), "table": _Held(table), "to": _Held(to),
-            "lens": _held_words(lens), "lens_out": _zeros(s, dtype=torch.int32), "weights": _Held(weights),
-            "weights_out": _zeros(*weights.shape), "status": _zeros(1, dtype=torch.int32),
-            "kept": _zeros(s, kvh, keep, dtype=torch.int32), "max_pages": max_pages, "pages": pages}
+    return {"k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)), "table": _Held(table), "to": _Held(to),
+            "lens": _Held(_words(lens)), "lens_out": _Held(_words([0] * s)), "weights": _Held(weights),
+            "weights_out": _Held(torch.zeros_like(weights)), "status": _Held(_words([0])),
+            "kept": _Held(torch.zeros(s, kvh, keep, dtype=torch.int32, device=_DEV)), "max_pages": max_pages, "pages": pages}
 
 
 def _prepare_copy(case, g):
@@ -344,9 +324,9 @@ def _prepare_copy(case, g):
     cap = max(lens)
     # every other sequence carries on from a third of its length
     runs = [(i, i, n // 3 if i % 2 else 0, n - (n // 3 if i % 2 else 0)) for i, n in enumerate(lens)]
-    dense = lambda: _normal(g, s, kvh, cap, hd, dtype=torch.float16)  # noqa: E731
-    return {"k": _pool(g, case, pages), "v": _pool(g, case, pages), "kc": dense(), "vc": dense(),
-            "table": _Held(table), "status": _zeros(1, dtype=torch.int32), "runs": runs, "runs_dev": _words(runs).long(),
+    dense = lambda: torch.randn(s, kvh, cap, hd, dtype=torch.float16, device=_DEV, generator=g)  # noqa: E731
+    return {"k": _Held(_pool(g, case, pages)), "v": _Held(_pool(g, case, pages)), "kc": _Held(dense()), "vc": _Held(dense()),
+            "table": _Held(table), "status": _Held(_words([0])), "runs": runs, "runs_dev": _words(runs).long(),
             "rows": sum(r[3] for r in runs), "cap": cap, "max_pages": max_pages, "pages": pages}
 
 
@@ -362,13 +342,13 @@ def _prepare_choose(case, g):
     log = torch.where(half, torch.gather(common, 1, pick), rare).to(torch.int32)
     pen = torch.stack([1 + 0.3 * torch.rand(r, device=_DEV, generator=g), 0.5 * torch.rand(r, device=_DEV, generator=g),
                        0.2 * torch.rand(r, device=_DEV, generator=g)], 1)
-    st = {"x": _normal(g, r, n, std=4.0), "y": _zeros(r, n),
-          "log": _Held(log), "pos": _held_words([v - 1 for v in hist]), "prompt": _held_words([v // 2 for v in hist]),
+    st = {"x": _Held(4 * torch.randn(r, n, device=_DEV, generator=g)), "y": _Held(torch.zeros(r, n, device=_DEV)),
+          "log": _Held(log), "pos": _Held(_words([v - 1 for v in hist])), "prompt": _Held(_words([v // 2 for v in hist])),
           "pen": _Held(pen.contiguous()), "stride": stride}
     if nb:
         st["bias_ids"] = _Held(torch.randint(0, n, (r, nb), device=_DEV, generator=g).to(torch.int32))
         st["bias"] = _Held(3 * torch.randn(r, nb, device=_DEV, generator=g))
-        st["bias_n"] = _held_words([max(0, nb - 3 * (i % 5)) for i in range(r)])
+        st["bias_n"] = _Held(_words([max(0, nb - 3 * (i % 5)) for i in range(r)]))
     if case["mask"]:
         words = -(-n // 32)
         # a grammar allows a few tokens in some states and almost all of them inside a string
@@ -378,7 +358,7 @@ def _prepare_choose(case, g):
         st["mask"] = _Held(torch.where(wide, torch.full_like(few, -1), few).to(torch.int32))
     if own:
         from tuckmill_b200 import cuda
-        st["partial"] = _Workspace(r * cuda.LOGITS_PARTIAL_BYTES)
+        st["partial"] = _Storage.take(r * cuda.LOGITS_PARTIAL_BYTES)
     return st
 
 
