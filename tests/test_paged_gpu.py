@@ -321,6 +321,18 @@ def test_small_weights_beside_a_large_one(ctx, hd, octaves):
     t.check()
 
 
+@pytest.mark.parametrize("hd,kvh", [(32, 32), (64, 16), (128, 8), (256, 4)])
+def test_the_stored_key_is_right_in_every_bit(ctx, hd, kvh):
+    """The new key in f16 is the definition's value in 64 bits, held in f32 and rounded to f16."""
+    t = Paged(ctx, [i % 20 for i in range(64)], kvh, kvh, hd, 16, dropped=70001, seed=16)
+    t.call()
+    ctx.fence()
+    k = f16(t.bk, t.k.shape)
+    for s, n in enumerate(t.lens):
+        want, _ = t.turned(t.qkv[s, kvh * hd:2 * kvh * hd].reshape(kvh, hd), t.kn, t.pos[s])
+        np.testing.assert_array_equal(k[t.table[s, n // 16], :, n % 16], want.astype(np.float32).astype(np.float16))
+
+
 def test_a_full_sequence_and_a_bad_page(ctx):
     t = Paged(ctx, [64, 30, 20], 4, 2, 64, 16, max_pages=4, seed=7)
     t.call()

@@ -187,10 +187,43 @@ struct cursor {
 
 // The vectors: a warp norms and rotates one query head, or a KV head's new key, and stores it.  Its latency is hidden by
 // nothing, so everything it needs is asked for at once.
+//
+// y / rms(y) * w, then the pairs (i, i + half) turned, in T; `row` is the warp's.
+__device__ __forceinline__ float inverse_rms(float mean, float eps) { return 1.0f / sqrtf(mean + eps); }
+__device__ __forceinline__ double inverse_rms(double mean, float eps) { return rsqrt(mean + (double)eps); }
+__device__ __forceinline__ void sine_cosine(float x, float &s, float &c) { sincosf(x, &s, &c); }
+__device__ __forceinline__ void sine_cosine(float x, double &s, double &c) { sincos((double)x, &s, &c); }
+template <int HD, typename T, int EPL, int PAIRS>
+__device__ __forceinline__ void norm_and_turn(T *row, const float (&y)[EPL], const float (&w)[EPL], const float (&freq)[PAIRS], float pos,
+                                              uint32_t half, float eps) {
+    const uint32_t lane = threadIdx.x & 31u;
+    T ss = 0;
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) ss += (T)y[r] * (T)y[r];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const T inv = inverse_rms(ss / (T)HD, eps);
+#pragma unroll
+    for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = (T)y[r] * inv * (T)w[r];
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < PAIRS; ++r) {
+        const uint32_t i = lane + 32 * r;
+        if (i < half) {
+            T sn, c;
+            sine_cosine(pos * freq[r], sn, c);
+            const T x0 = row[i], x1 = row[i + half];
+            row[i] = x0 * c - x1 * sn;
+            row[i + half] = x0 * sn + x1 * c;
+        }
+    }
+    __syncwarp();
+}
+
 template <int HD>
 __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const paged_args a) {
     constexpr int EPL = HD / 32;
-    __shared__ float rows[8][HD];
+    __shared__ double rows[8][HD];
     tmdev::pdl_wait();
     tmdev::pdl_trigger();  // the next kernel may read what those before this one have written
     const uint32_t warp = tmdev::warp_index(), lane = threadIdx.x & 31u, per = a.heads + a.kv_heads;
@@ -203,7 +236,7 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
     const float *nw = is_k ? a.k_norm : a.q_norm, *vs = a.v + (size_t)s * a.kv_stride + (size_t)kvh * HD;
     const uint32_t half = a.n_rot / 2u;
     constexpr int kPairs = HD > 64 ? HD / 64 : 1;  // rotation pairs of a lane, at most
-    float y[EPL], w[EPL], v[EPL], freq[kPairs], ss = 0.0f;
+    float y[EPL], w[EPL], v[EPL], freq[kPairs];
 #pragma unroll
     for (int r = 0; r < EPL; ++r) {
         y[r] = src[lane + 32 * r];
@@ -217,40 +250,26 @@ __global__ void __launch_bounds__(256) attention_paged_vectors_kernel(const page
         if (x == 0u && lane == 0 && len != kSeqNone) atomicOr(a.status, TM_CUDA_STATUS_PAST_CAPACITY);
         return;
     }
-#pragma unroll
-    for (int r = 0; r < EPL; ++r) ss = fmaf(y[r], y[r], ss);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
-    float *row = rows[warp];
-#pragma unroll
-    for (int r = 0; r < EPL; ++r) row[lane + 32 * r] = y[r] * inv * w[r];
-    __syncwarp();
-#pragma unroll
-    for (int r = 0; r < kPairs; ++r) {
-        const uint32_t i = lane + 32 * r;
-        if (i < half) {
-            float sn, c;
-            sincosf((float)pos * freq[r], &sn, &c);
-            const float x0 = row[i], x1 = row[i + half];
-            row[i] = x0 * c - x1 * sn;
-            row[i + half] = x0 * sn + x1 * c;
-        }
-    }
-    __syncwarp();
     if (is_k) {
         if (id >= a.pages) {
             if (lane == 0) atomicOr(a.status, TM_CUDA_STATUS_BAD_PAGE);
             return;
         }
+        // The stored key is what every later token meets: worked out in 64 bits, so that what is rounded to f16 is right in every bit
+        // of f32.  (In 32 bits one element in some thousands comes to lie on the other side of a tie of f16, and a whole step of it
+        // away.  The queries' warps take as long, so this costs nothing.)
+        double *row = rows[warp];
+        norm_and_turn<HD>(row, y, w, freq, (float)pos, half, a.eps);
         const size_t to = ((((size_t)id * a.kv_heads + kvh) << a.page_log) + (len & ((1u << a.page_log) - 1u))) * HD;
 #pragma unroll
         for (int r = 0; r < EPL; ++r) {
-            a.kp[to + lane + 32 * r] = __float2half_rn(row[lane + 32 * r]);
+            a.kp[to + lane + 32 * r] = __float2half_rn((float)row[lane + 32 * r]);
             a.vp[to + lane + 32 * r] = __float2half_rn(v[r]);
         }
         return;
     }
+    float *row = (float *)rows[warp];
+    norm_and_turn<HD>(row, y, w, freq, (float)pos, half, a.eps);
     float top = 0.0f;
 #pragma unroll
     for (int r = 0; r < EPL; ++r) top = fmaxf(top, fabsf(row[lane + 32 * r]));
