@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<u
 // it.  Three launches: the vectors (queries and new rows: norm, rotation, f16), the rows, and the join of what the warps
 // have found.  The second starts beside the first and waits for it when it has its rows on their way.
 //
-// What it measured (8 KV heads of 128): the rows of one sequence of 131071 (537 MB) 84 us, 6.4 TB/s, of 32 up to 4095 (343 MB
+// What it measured (8 KV heads of 128): the rows of one sequence of 131071 (537 MB) 85 us, 6.3 TB/s, of 32 up to 4095 (343 MB
 // with the scores) 61 us, 5.7 TB/s; around them 3 us until the first rows arrive and 3 to 7 us of the join.  (Slices whose
 // last eighth went to whichever warp was free measured the same: what ends late waits for the memory, not for work.)
 //
